@@ -71,7 +71,7 @@ def build_bench(force=False):
 
 
 GLUE = {"libmtpr_bind.so": ["mtpr_bind.cpp"], "libnep_bind.so": ["nep_bind.cpp"], "libfvt_sr_op_bind.so": ["fvt_sr_op_bind.cpp"],
-        "libfitutils_bind.so": ["fitutils_bind.cpp"]}
+        "libfitutils_bind.so": ["fitutils_bind.cpp"], "libfitnet_bind.so": ["fitnet_bind.cpp"]}
 
 
 def build_glue(force=False, verbose=False):

@@ -1,0 +1,59 @@
+// Types and small device helpers shared by the fitting-network kernels (route.cu, dense.cu, orthogonalize.cu).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "common.cuh"
+
+namespace ai2b {
+
+using bf16 = __nv_bfloat16;
+using f16 = __half;
+
+// Arithmetic is done in float whatever the element type; a result is rounded once, when it is stored.
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(f16 v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 from_float<bf16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ f16 from_float<f16>(float v) { return __float2half_rn(v); }
+
+// N consecutive elements that are loaded and stored at once (the address is a multiple of their size)
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+inline size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+inline size_t element_bytes(int dtype) { return dtype == AI2B_F32 ? 4 : 2; }
+inline bool known_dtype(int dtype) { return dtype == AI2B_F32 || dtype == AI2B_BF16 || dtype == AI2B_F16; }
+
+// f(T{}) with the element type of `dtype` (checked by the caller)
+template <typename F>
+inline int with_type(int dtype, F &&f)
+{
+    if (dtype == AI2B_F32) return f(float{});
+    if (dtype == AI2B_BF16) return f(bf16{});
+    return f(f16{});
+}
+
+// Largest power of two <= 16 that divides every number given: the bytes that one access may move
+template <typename... N>
+inline int common_alignment(N... n)
+{
+    const unsigned long long all = (0ull | ... | (unsigned long long)n) | 16ull;
+    return (int)(all & (~all + 1));
+}
+
+// Offsets come from device memory that the host has not seen: whatever they hold, the rows of group e are [begin, end) inside [0, rows].
+struct RowRange {
+    long long begin, end;
+};
+__device__ __forceinline__ RowRange group_rows(const int *offsets, int e, long long rows)
+{
+    if (!offsets) return RowRange{0, rows};
+    const long long b = min((long long)max(offsets[e], 0), rows), n = min((long long)max(offsets[e + 1], 0), rows);
+    return RowRange{b, n > b ? n : b};
+}
+
+}  // namespace ai2b

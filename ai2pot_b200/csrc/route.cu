@@ -1,0 +1,423 @@
+// Rows sorted by network and back: the plan (a stable counting sort of the slots by network), the copy into sorted order, the
+// weighted sum back, and the gradients of both.
+//
+//   slot s = t * k + j is entry j of token (atom) t; key_s = index[s] if 0 <= index[s] < E, else E (dropped)
+//   order    slots sorted by (key, slot); dropped ones come last and are written as -1 - s
+//   position position[s] = row of slot s in that order, -1 if dropped;  offsets[e] = number of slots with key < e
+//   dispatch xs[r] = x[order[r] / k], zero where dropped            (gradient: the weighted sum below with weights of one)
+//   combine  y[t] = sum_j w[t,j] ys[position[t,j]]                  (sums in float, j ascending: no atomics, same bits every time)
+//   combine's gradient  gys[position[s]] = w[s] gy[t], gw[s] = <gy[t], ys[position[s]]>, zero for dropped slots and rows
+//
+// All of it moves bytes: each row is read and written once, in accesses of up to 16 bytes by neighbouring lanes.
+#include "fitnet.cuh"
+
+namespace ai2b {
+
+constexpr int PLAN_WARPS = 32;            // warps of a plan block; each walks its own run of consecutive slots
+constexpr int MAX_EXPERTS = 1024;         // a block holds PLAN_WARPS + 1 rows of E + 1 counters: 135 KB of shared memory at the limit
+
+template <typename I>
+__device__ __forceinline__ int slot_key(const I *index, long long s, int E)
+{
+    const I e = index[s];
+    return e >= 0 && e < (I)E ? (int)e : E;
+}
+
+// Counts of one warp's run of slots, kept in its own row of shared memory: lanes with the same key are found by a vote, and the
+// first of them adds for all.
+template <typename I>
+__device__ __forceinline__ void count_run(const I *index, long long begin, long long end, int E, int *counts, int lane)
+{
+    for (long long s0 = begin; s0 < end; s0 += 32) {
+        const bool in = s0 + lane < end;
+        const int key = in ? slot_key(index, s0 + lane, E) : E + 1;
+        const unsigned same = __match_any_sync(FULL_MASK, key);
+        if (in && (same & ((1u << lane) - 1)) == 0) counts[key] += __popc(same);
+        __syncwarp();
+    }
+}
+
+// [E + 1][gridDim.x] counts of each block's run
+template <typename I>
+__global__ void __launch_bounds__(PLAN_WARPS * 32) route_count_kernel(const I *__restrict__ index, long long nslots, long long run, int E, int *__restrict__ block_counts)
+{
+    extern __shared__ int counts[];      // [PLAN_WARPS][E + 1]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < PLAN_WARPS * (E + 1); i += blockDim.x) counts[i] = 0;
+    __syncthreads();
+    chain_wait();
+    chain_release();
+    const long long begin = ((long long)blockIdx.x * PLAN_WARPS + warp) * run, end = min(begin + run, nslots);
+    count_run(index, begin, end, E, counts + warp * (E + 1), lane);
+    __syncthreads();
+    for (int e = threadIdx.x; e <= E; e += blockDim.x) {
+        int n = 0;
+        for (int w = 0; w < PLAN_WARPS; w++) n += counts[w * (E + 1) + e];
+        block_counts[(size_t)e * gridDim.x + blockIdx.x] = n;
+    }
+}
+
+// Row of every slot: slots of smaller keys, of the same key in earlier blocks, in earlier warps, and in earlier lanes.
+template <typename I>
+__global__ void __launch_bounds__(PLAN_WARPS * 32)
+route_place_kernel(const I *__restrict__ index, long long nslots, long long run, int E, const int *__restrict__ block_counts, int *__restrict__ order,
+                   int *__restrict__ position, int *__restrict__ offsets)
+{
+    extern __shared__ int counts[];      // [PLAN_WARPS][E + 1], then the first row of each key
+    __shared__ int warp_total[PLAN_WARPS];
+    int *first = counts + PLAN_WARPS * (E + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < PLAN_WARPS * (E + 1); i += blockDim.x) counts[i] = 0;
+    __syncthreads();
+    chain_wait();
+    chain_release();
+    const long long begin = ((long long)blockIdx.x * PLAN_WARPS + warp) * run, end = min(begin + run, nslots);
+    int *mine = counts + warp * (E + 1);
+    count_run(index, begin, end, E, mine, lane);
+    __syncthreads();
+    // totals of every key, and what earlier blocks hold of it (a single block has its own counts only)
+    int before = 0;
+    for (int e = warp; e <= E; e += PLAN_WARPS) {
+        int total = 0, earlier = 0;
+        if (gridDim.x == 1) {
+            total = counts[lane * (E + 1) + e];
+        } else {
+            for (int b = lane; b < (int)gridDim.x; b += 32) {
+                const int n = block_counts[(size_t)e * gridDim.x + b];
+                total += n;
+                earlier += b < (int)blockIdx.x ? n : 0;
+            }
+        }
+        total = warp_sum(total);
+        earlier = warp_sum(earlier);
+        if (lane == 0) first[e] = total;
+        // counts become each warp's exclusive prefix within the key, from `earlier` on
+        int c = counts[lane * (E + 1) + e];
+        const int own = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(FULL_MASK, c, o);
+            if (lane >= o) c += up;
+        }
+        counts[lane * (E + 1) + e] = earlier + c - own;
+    }
+    __syncthreads();
+    // exclusive prefix of the totals over the keys (E + 1 <= 1025: two at most per thread)
+    const int per = (E + 1 + (int)blockDim.x - 1) / (int)blockDim.x, e0 = threadIdx.x * per;
+    int sum = 0;
+    for (int e = e0; e < min(e0 + per, E + 1); e++) sum += first[e];
+    int scan = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(FULL_MASK, scan, o);
+        if (lane >= o) scan += up;
+    }
+    if (lane == 31) warp_total[warp] = scan;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) before += warp_total[w];
+    before += scan - sum;
+    for (int e = e0; e < min(e0 + per, E + 1); e++) {
+        const int n = first[e];
+        first[e] = before;
+        if (blockIdx.x == 0) offsets[e] = before;
+        before += n;
+    }
+    __syncthreads();
+    for (long long s0 = begin; s0 < end; s0 += 32) {
+        const long long s = s0 + lane;
+        const bool in = s < end;
+        const int key = in ? slot_key(index, s, E) : E + 1;
+        const unsigned same = __match_any_sync(FULL_MASK, key), lower = same & ((1u << lane) - 1);
+        if (in) {
+            const int row = first[key] + mine[key] + __popc(lower);
+            order[row] = key < E ? (int)s : -1 - (int)s;
+            position[s] = key < E ? row : -1;
+        }
+        __syncwarp();
+        if (in && lower == 0) mine[key] += __popc(same);
+        __syncwarp();
+    }
+}
+
+// i / d; a division of 64-bit numbers takes several times as long as the rest of a thread's arithmetic, so it is made of 32 bits where
+// the whole range fits
+__device__ __forceinline__ long long row_of(long long i, int d, bool narrow) { return narrow ? (long long)((unsigned)i / (unsigned)d) : i / d; }
+
+// Thread i of the grid moves access i % per_row of row i / per_row, then the same UNROLL - 1 more times a grid further on: that many
+// loads are in flight at once.
+template <typename V, int UNROLL>
+__global__ void __launch_bounds__(256) dispatch_kernel(V *__restrict__ out, const V *__restrict__ x, long long x_stride, const int *__restrict__ order, long long rows, int k,
+                                int per_row)
+{
+    chain_wait();
+    chain_release();
+    const long long total = rows * per_row, step = (long long)gridDim.x * blockDim.x;
+    const bool narrow = total <= 0xffffffffLL;
+    for (long long i0 = (long long)blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += UNROLL * step) {
+        V v[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long i = i0 + u * step;
+            v[u] = V{};
+            if (i < total) {
+                const long long r = row_of(i, per_row, narrow);
+                const int s = order[r];
+                if (s >= 0 && s < rows) v[u] = x[(long long)(s / k) * x_stride + (int)(i - r * per_row)];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++)
+            if (i0 + u * step < total) out[i0 + u * step] = v[u];
+    }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(256) combine_kernel(Pack<T, N> *__restrict__ y, const Pack<T, N> *__restrict__ ys, long long ys_stride, const float *__restrict__ weights,
+                               const int *__restrict__ position, long long tokens, int k, int per_row, long long rows)
+{
+    chain_wait();
+    chain_release();
+    const long long total = tokens * per_row, step = (long long)gridDim.x * blockDim.x;
+    const bool narrow = total <= 0xffffffffLL;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const long long t = row_of(i, per_row, narrow);
+        const int c = (int)(i - t * per_row);
+        float sum[N] = {};
+        for (int j0 = 0; j0 < k; j0 += 4) {      // four rows in flight
+            Pack<T, N> v[4];
+            float w[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                w[u] = 0.f;
+                if (j0 + u < k) {
+                    const int p = position[t * k + j0 + u];
+                    if (p >= 0 && p < rows) {
+                        w[u] = weights ? weights[t * k + j0 + u] : 1.f;
+                        v[u] = ys[p * ys_stride + c];
+                    } else {
+                        v[u] = Pack<T, N>{};     // a dropped slot adds zero whatever its weight and rows hold
+                    }
+                } else {
+                    v[u] = Pack<T, N>{};
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int n = 0; n < N; n++) sum[n] = fmaf(w[u], to_float(v[u].v[n]), sum[n]);
+        }
+        Pack<T, N> out;
+#pragma unroll
+        for (int n = 0; n < N; n++) out.v[n] = from_float<T>(sum[n]);
+        y[i] = out;
+    }
+}
+
+// `lanes` neighbouring lanes (a power of two) take one token; gy[t] comes from memory for its first slot and from the L1 cache for
+// the others. The rows after the last network are zeroed by the whole grid.
+template <typename T, int N>
+__global__ void __launch_bounds__(256)
+combine_backward_kernel(Pack<T, N> *__restrict__ gys, float *__restrict__ gw, const Pack<T, N> *__restrict__ gy, long long gy_stride,
+                        const Pack<T, N> *__restrict__ ys, long long ys_stride, const float *__restrict__ weights, const int *__restrict__ position,
+                        const int *__restrict__ last_offset, long long tokens, int k, int per_row, int lanes)
+{
+    chain_wait();
+    chain_release();
+    const long long nslots = tokens * k, threads = (long long)gridDim.x * blockDim.x, me = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    const int part = threadIdx.x & (lanes - 1);
+    const unsigned group = lanes == 32 ? FULL_MASK : ((1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
+    for (long long t = me / lanes; t < tokens; t += threads / lanes) {
+        for (int j = 0; j < k; j++) {
+            const long long s = t * k + j;
+            const int p = position[s];
+            float dot = 0.f;
+            if (p >= 0 && p < nslots) {
+                const float w = weights[s];
+                for (int c = part; c < per_row; c += lanes) {
+                    const Pack<T, N> g = gy[t * gy_stride + c], v = ys[p * ys_stride + c];
+                    Pack<T, N> out;
+#pragma unroll
+                    for (int n = 0; n < N; n++) {
+                        const float gn = to_float(g.v[n]);
+                        dot = fmaf(gn, to_float(v.v[n]), dot);
+                        out.v[n] = from_float<T>(w * gn);
+                    }
+                    gys[(long long)p * per_row + c] = out;
+                }
+            }
+            for (int o = lanes >> 1; o >= 1; o >>= 1) dot += __shfl_xor_sync(group, dot, o);
+            if (part == 0) gw[s] = dot;
+        }
+    }
+    const long long first = min(max((long long)*last_offset, 0ll), nslots) * per_row;
+    for (long long i = first + me; i < nslots * per_row; i += threads) gys[i] = Pack<T, N>{};
+}
+
+// Blocks for `threads_wanted` threads of work: as many as are resident at once
+template <typename Kern>
+static int grid_for(KernelSetup &ks, Kern kern, long long threads_wanted, int *grid)
+{
+    int per_sm = 1;
+    const int rc = kernel_setup(ks, kern, 0, 256, &per_sm);
+    if (rc != AI2B_OK) return rc;
+    const long long blocks = (threads_wanted + 255) / 256, most = (long long)per_sm * sm_count();
+    *grid = (int)(blocks < 1 ? 1 : blocks < most ? blocks : most);
+    return AI2B_OK;
+}
+
+// One block walks up to 16384 slots by itself. More slots are cut into runs for two blocks per SM at most; with many networks fewer
+// blocks are taken, because each reads all blocks' counts (E + 1 of them per block).
+static int plan_blocks(long long nslots, int E)
+{
+    if (nslots <= 16384) return 1;
+    long long n = (nslots + 4095) / 4096;
+    const long long most = 2 * sm_count(), by_counts = 131072 / (E + 1);
+    if (n > most) n = most;
+    if (n > by_counts) n = by_counts;
+    return (int)n;
+}
+
+template <typename I>
+static int route_plan(const I *index, long long nslots, int E, int *order, int *position, int *offsets, int *counts, cudaStream_t st)
+{
+    const int blocks = plan_blocks(nslots, E);
+    const long long warps = (long long)blocks * PLAN_WARPS, run = ((nslots + warps - 1) / warps + 31) / 32 * 32;
+    const size_t smem = sizeof(int) * (size_t)(PLAN_WARPS + 1) * (E + 1);
+    int rc;
+    if (blocks > 1) {
+        static KernelSetup ks;
+        if ((rc = kernel_setup(ks, route_count_kernel<I>, smem)) != AI2B_OK) return rc;
+        AI2B_CUDA(launch_chained(route_count_kernel<I>, dim3(blocks), dim3(PLAN_WARPS * 32), smem, st, index, nslots, run, E, counts));
+    }
+    static KernelSetup ks;
+    if ((rc = kernel_setup(ks, route_place_kernel<I>, smem)) != AI2B_OK) return rc;
+    AI2B_CUDA(launch_chained(route_place_kernel<I>, dim3(blocks), dim3(PLAN_WARPS * 32), smem, st, index, nslots, run, E, (const int *)counts, order, position, offsets));
+    return AI2B_OK;
+}
+
+template <typename V>
+static int dispatch_rows(void *xs, const void *x, long long x_stride_bytes, const int *order, long long rows, int k, long long row_bytes, cudaStream_t st)
+{
+    static KernelSetup ks;
+    const int per_row = (int)(row_bytes / sizeof(V));
+    const long long total = rows * per_row;
+    // below 4 accesses per resident thread one at a time: more threads share the latency
+    int grid, rc;
+    if (total <= (long long)sm_count() * 2048) {
+        if ((rc = grid_for(ks, dispatch_kernel<V, 1>, total, &grid)) != AI2B_OK) return rc;
+        AI2B_CUDA(launch_chained(dispatch_kernel<V, 1>, dim3(grid), dim3(256), 0, st, (V *)xs, (const V *)x, x_stride_bytes / (long long)sizeof(V), order, rows, k, per_row));
+    } else {
+        static KernelSetup ks4;
+        if ((rc = grid_for(ks4, dispatch_kernel<V, 4>, (total + 3) / 4, &grid)) != AI2B_OK) return rc;
+        AI2B_CUDA(launch_chained(dispatch_kernel<V, 4>, dim3(grid), dim3(256), 0, st, (V *)xs, (const V *)x, x_stride_bytes / (long long)sizeof(V), order, rows, k, per_row));
+    }
+    return AI2B_OK;
+}
+
+// f(T{}, integral_constant<N>) for the number of elements that one access of `bytes` bytes holds
+template <typename F>
+static int with_pack(int dtype, int bytes, F &&f)
+{
+    return with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (bytes >= 16) return f(t, std::integral_constant<int, 16 / (int)sizeof(T)>{});
+        if (bytes >= 8) return f(t, std::integral_constant<int, 8 / (int)sizeof(T)>{});
+        if (bytes >= 4) return f(t, std::integral_constant<int, 4 / (int)sizeof(T)>{});
+        return f(t, std::integral_constant<int, 1>{});
+    });
+}
+
+static int check_rows(const char *what, int dtype, long long tokens, int k, int width)
+{
+    AI2B_REQUIRE(known_dtype(dtype), AI2B_ERR_INVALID, "%s: unknown element type %d", what, dtype);
+    AI2B_REQUIRE(tokens >= 0 && k >= 1 && width >= 1, AI2B_ERR_INVALID, "%s: tokens %lld, k %d, width %d", what, tokens, k, width);
+    AI2B_REQUIRE(tokens <= 0x7fffffffLL / k, AI2B_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 slots", what);
+    return AI2B_OK;
+}
+
+}  // namespace ai2b
+
+using namespace ai2b;
+
+extern "C" size_t ai2b_route_workspace_bytes(long long tokens, int k, int experts)
+{
+    if (tokens < 0 || k < 1 || experts < 1 || experts > MAX_EXPERTS) return 0;
+    return sizeof(int) * (size_t)plan_blocks(tokens * k, experts) * (experts + 1);
+}
+
+extern "C" int ai2b_route(const void *d_index, int index_is_i64, long long tokens, int k, int experts, int *d_order, int *d_position, int *d_offsets,
+                          void *d_workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = check_rows("ai2b_route", AI2B_F32, tokens, k, 1);
+    if (rc != AI2B_OK) return rc;
+    AI2B_REQUIRE(experts >= 1, AI2B_ERR_INVALID, "ai2b_route: experts must be positive (got %d)", experts);
+    AI2B_REQUIRE(experts <= MAX_EXPERTS, AI2B_ERR_UNSUPPORTED, "ai2b_route: at most %d experts (got %d)", MAX_EXPERTS, experts);
+    const long long nslots = tokens * k;
+    AI2B_REQUIRE(d_offsets && (nslots == 0 || (d_index && d_order && d_position)), AI2B_ERR_INVALID, "ai2b_route: NULL pointer");
+    AI2B_REQUIRE(d_workspace && workspace_bytes >= ai2b_route_workspace_bytes(tokens, k, experts), AI2B_ERR_WORKSPACE, "ai2b_route: workspace of %zu bytes, %zu needed",
+                 workspace_bytes, ai2b_route_workspace_bytes(tokens, k, experts));
+    cudaStream_t st = (cudaStream_t)stream;
+    return index_is_i64 ? route_plan((const long long *)d_index, nslots, experts, d_order, d_position, d_offsets, (int *)d_workspace, st)
+                        : route_plan((const int *)d_index, nslots, experts, d_order, d_position, d_offsets, (int *)d_workspace, st);
+}
+
+extern "C" int ai2b_route_dispatch(int dtype, void *d_xs, const void *d_x, long long x_stride, const int *d_order, long long tokens, int k, int width, void *stream)
+{
+    int rc = check_rows("ai2b_route_dispatch", dtype, tokens, k, width);
+    if (rc != AI2B_OK || tokens == 0) return rc;
+    AI2B_REQUIRE(d_xs && d_x && d_order, AI2B_ERR_INVALID, "ai2b_route_dispatch: NULL pointer");
+    AI2B_REQUIRE(x_stride >= width || tokens == 1, AI2B_ERR_INVALID, "ai2b_route_dispatch: row stride %lld below the width %d", x_stride, width);
+    const long long size = (long long)element_bytes(dtype), row = size * width, stride = size * x_stride;
+    const int bytes = common_alignment(d_xs, d_x, row, stride);
+    cudaStream_t st = (cudaStream_t)stream;
+    const long long rows = tokens * k;
+    if (bytes >= 16) return dispatch_rows<uint4>(d_xs, d_x, stride, d_order, rows, k, row, st);
+    if (bytes >= 8) return dispatch_rows<uint2>(d_xs, d_x, stride, d_order, rows, k, row, st);
+    if (bytes >= 4) return dispatch_rows<unsigned>(d_xs, d_x, stride, d_order, rows, k, row, st);
+    return dispatch_rows<unsigned short>(d_xs, d_x, stride, d_order, rows, k, row, st);
+}
+
+extern "C" int ai2b_route_combine(int dtype, void *d_y, const void *d_ys, long long ys_stride, const float *d_weights, const int *d_position, long long tokens, int k,
+                                  int width, void *stream)
+{
+    int rc = check_rows("ai2b_route_combine", dtype, tokens, k, width);
+    if (rc != AI2B_OK || tokens == 0) return rc;
+    AI2B_REQUIRE(d_y && d_ys && d_position, AI2B_ERR_INVALID, "ai2b_route_combine: NULL pointer");
+    AI2B_REQUIRE(ys_stride >= width, AI2B_ERR_INVALID, "ai2b_route_combine: row stride %lld below the width %d", ys_stride, width);
+    const long long size = (long long)element_bytes(dtype);
+    return with_pack(dtype, common_alignment(d_y, d_ys, size * width, size * ys_stride), [&](auto t, auto n) {
+        using T = decltype(t);
+        constexpr int N = decltype(n)::value;
+        static KernelSetup ks;
+        int grid;
+        const int rc2 = grid_for(ks, combine_kernel<T, N>, tokens * (width / N), &grid);
+        if (rc2 != AI2B_OK) return rc2;
+        AI2B_CUDA(launch_chained(combine_kernel<T, N>, dim3(grid), dim3(256), 0, (cudaStream_t)stream, (Pack<T, N> *)d_y, (const Pack<T, N> *)d_ys, ys_stride / N, d_weights,
+                                 d_position, tokens, k, width / N, tokens * k));
+        return (int)AI2B_OK;
+    });
+}
+
+extern "C" int ai2b_route_combine_backward(int dtype, void *d_gys, float *d_gweights, const void *d_gy, long long gy_stride, const void *d_ys, long long ys_stride,
+                                           const float *d_weights, const int *d_position, const int *d_offsets, long long tokens, int k, int experts, int width,
+                                           void *stream)
+{
+    int rc = check_rows("ai2b_route_combine_backward", dtype, tokens, k, width);
+    if (rc != AI2B_OK || tokens == 0) return rc;
+    AI2B_REQUIRE(d_gys && d_gweights && d_gy && d_ys && d_weights && d_position && d_offsets, AI2B_ERR_INVALID, "ai2b_route_combine_backward: NULL pointer");
+    AI2B_REQUIRE(experts >= 1 && ys_stride >= width && (gy_stride >= width || tokens == 1), AI2B_ERR_INVALID,
+                 "ai2b_route_combine_backward: experts %d, width %d, row strides %lld and %lld", experts, width, ys_stride, gy_stride);
+    const long long size = (long long)element_bytes(dtype);
+    return with_pack(dtype, common_alignment(d_gys, d_gy, d_ys, size * width, size * ys_stride, size * gy_stride), [&](auto t, auto n) {
+        using T = decltype(t);
+        constexpr int N = decltype(n)::value;
+        static KernelSetup ks;
+        const int per_row = width / N, lanes = per_row >= 32 ? 32 : pow2ceil(per_row);
+        int grid;
+        const int rc2 = grid_for(ks, combine_backward_kernel<T, N>, tokens * lanes, &grid);
+        if (rc2 != AI2B_OK) return rc2;
+        AI2B_CUDA(launch_chained(combine_backward_kernel<T, N>, dim3(grid), dim3(256), 0, (cudaStream_t)stream, (Pack<T, N> *)d_gys, d_gweights, (const Pack<T, N> *)d_gy,
+                                 gy_stride / N, (const Pack<T, N> *)d_ys, ys_stride / N, d_weights, d_position, d_offsets + experts, tokens, k, per_row, lanes));
+        return (int)AI2B_OK;
+    });
+}

@@ -1,0 +1,329 @@
+// libfitnet_bind.so: fitnet::routeOp, dispatchOp, combineOp, denseOp, orthogonalizeOp over the C ABI (the fitting-network section of
+// include/ai2pot_b200.h). dispatchOp, combineOp and denseOp are differentiable once: a backward pass that is asked to build a graph of
+// itself (create_graph=True) is refused, because that graph would lack these gradients.
+#include "glue_common.h"
+
+using namespace ai2b_glue;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+int dtype_of(const at::Tensor &t, const char *name)
+{
+    require_cuda(t, name);
+    switch (t.scalar_type()) {
+    case at::kFloat: return AI2B_F32;
+    case at::kBFloat16: return AI2B_BF16;
+    case at::kHalf: return AI2B_F16;
+    default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16 (got ", t.scalar_type(), ")");
+    }
+}
+
+void require_like(const at::Tensor &t, const at::Tensor &like, const char *name)
+{
+    require_cuda(t, name);
+    TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), " (got ", t.device(), ")");
+    TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must be ", like.scalar_type(), " (got ", t.scalar_type(), ")");
+}
+
+// A matrix whose rows are contiguous and do not overlap: what the kernels take, with any row stride. Other layouts (transposed or
+// expanded tensors) are copied.
+at::Tensor rows_of(const at::Tensor &t)
+{
+    const bool fits = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+    return fits ? t : t.contiguous();
+}
+int64_t row_stride(const at::Tensor &t) { return t.size(0) <= 1 ? std::max<int64_t>(t.size(1), 1) : t.stride(0); }
+
+void require_first_order(const char *name)
+{
+    TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: create_graph=True is not supported");
+}
+
+std::optional<at::Tensor> given(const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+
+bool wants_grad(std::initializer_list<const at::Tensor *> ts)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor *t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// ---- rows sorted by network -------------------------------------------------------------------------------------------------
+
+variable_list route(const at::Tensor &index, int64_t experts)
+{
+    require_cuda(index, "index");
+    TORCH_CHECK(index.scalar_type() == at::kInt || index.scalar_type() == at::kLong, "index must be int32 or int64 (got ", index.scalar_type(), ")");
+    TORCH_CHECK(index.dim() == 1 || index.dim() == 2, "index must be [tokens] or [tokens, k]");
+    TORCH_CHECK(experts >= 1 && experts <= 1024, "experts must be between 1 and 1024 (got ", experts, ")");
+    c10::cuda::CUDAGuard guard(index.device());
+    const at::Tensor idx = index.contiguous();
+    const int64_t tokens = idx.size(0), k = idx.dim() == 2 ? idx.size(1) : 1;
+    TORCH_CHECK(k >= 1 && k <= 0x7fffffff, "index needs one column at least");
+    const auto opt = idx.options().dtype(at::kInt);
+    at::Tensor order = at::empty({tokens * k}, opt), position = at::empty({tokens, k}, opt), offsets = at::empty({experts + 1}, opt);
+    const size_t bytes = ai2b_route_workspace_bytes(tokens, (int)k, (int)experts);
+    at::Tensor ws = workspace(bytes, idx);
+    check(ai2b_route(idx.data_ptr(), idx.scalar_type() == at::kLong, tokens, (int)k, (int)experts, order.data_ptr<int>(), position.data_ptr<int>(), offsets.data_ptr<int>(),
+                     ws.data_ptr(), bytes, stream()),
+          "ai2b_route");
+    return {order, position, offsets};
+}
+
+struct Plan {
+    int64_t tokens, k, experts;
+};
+Plan check_plan(const at::Tensor &like, const at::Tensor &order, const at::Tensor &position, const at::Tensor &offsets)
+{
+    for (const at::Tensor *t : {&order, &position, &offsets}) {
+        iptr(*t, "the route's tensors");
+        TORCH_CHECK(t->device() == like.device(), "the route is on ", t->device(), ", the rows on ", like.device());
+    }
+    TORCH_CHECK(position.dim() == 2 && position.size(1) >= 1 && order.dim() == 1 && order.size(0) == position.numel() && offsets.dim() == 1 && offsets.size(0) >= 2,
+                "order [tokens * k], position [tokens, k] and offsets [experts + 1] are those of one route");
+    return Plan{position.size(0), position.size(1), offsets.size(0) - 1};
+}
+
+at::Tensor combine_rows(const at::Tensor &ys_any, const float *weights, const at::Tensor &position)
+{
+    const at::Tensor ys = rows_of(ys_any);
+    at::Tensor y = at::empty({position.size(0), ys.size(1)}, ys.options());
+    check(ai2b_route_combine(dtype_of(ys, "ys"), y.data_ptr(), ys.data_ptr(), row_stride(ys), weights, position.data_ptr<int>(), position.size(0), (int)position.size(1),
+                             (int)ys.size(1), stream()),
+          "ai2b_route_combine");
+    return y;
+}
+
+at::Tensor dispatch_rows(const at::Tensor &x_any, const at::Tensor &order, const Plan &p)
+{
+    const at::Tensor x = rows_of(x_any);
+    at::Tensor xs = at::empty({p.tokens * p.k, x.size(1)}, x.options());
+    check(ai2b_route_dispatch(dtype_of(x, "x"), xs.data_ptr(), x.data_ptr(), row_stride(x), order.data_ptr<int>(), p.tokens, (int)p.k, (int)x.size(1), stream()),
+          "ai2b_route_dispatch");
+    return xs;
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &order, const at::Tensor &position, const Plan &p)
+    {
+        ctx->save_for_backward({position});
+        return dispatch_rows(x, order, p);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        require_first_order("dispatch");
+        c10::cuda::CUDAGuard guard(grads[0].device());
+        return {combine_rows(grads[0], nullptr, ctx->get_saved_variables()[0]), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &ys, const at::Tensor &weights, const at::Tensor &position, const at::Tensor &offsets)
+    {
+        ctx->save_for_backward({ys, weights, position, offsets});
+        return combine_rows(ys, weights.data_ptr<float>(), position);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        require_first_order("combine");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor ys = rows_of(saved[0]), &weights = saved[1], &position = saved[2], &offsets = saved[3], gy = rows_of(grads[0]);
+        c10::cuda::CUDAGuard guard(ys.device());
+        at::Tensor gys = at::empty(ys.sizes(), ys.options()), gw = at::empty(weights.sizes(), weights.options());
+        check(ai2b_route_combine_backward(dtype_of(ys, "ys"), gys.data_ptr(), gw.data_ptr<float>(), gy.data_ptr(), row_stride(gy), ys.data_ptr(), row_stride(ys),
+                                          weights.data_ptr<float>(), position.data_ptr<int>(), offsets.data_ptr<int>(), position.size(0), (int)position.size(1),
+                                          (int)offsets.size(0) - 1, (int)ys.size(1), stream()),
+              "ai2b_route_combine_backward");
+        return {gys, gw, at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor dispatch(const at::Tensor &x, const at::Tensor &order, const at::Tensor &position, const at::Tensor &offsets)
+{
+    dtype_of(x, "x");
+    const Plan p = check_plan(x, order, position, offsets);
+    TORCH_CHECK(x.dim() == 2 && x.size(0) == p.tokens && x.size(1) >= 1, "x must be [", p.tokens, ", width] (got ", x.sizes(), ")");
+    c10::cuda::CUDAGuard guard(x.device());
+    return wants_grad({&x}) ? Dispatch::apply(x, order, position, p) : dispatch_rows(x, order, p);
+}
+
+at::Tensor combine(const at::Tensor &ys, const at::Tensor &weights_any, const at::Tensor &order, const at::Tensor &position, const at::Tensor &offsets)
+{
+    dtype_of(ys, "ys");
+    const Plan p = check_plan(ys, order, position, offsets);
+    TORCH_CHECK(ys.dim() == 2 && ys.size(0) == p.tokens * p.k && ys.size(1) >= 1, "ys must be [", p.tokens * p.k, ", width] (got ", ys.sizes(), ")");
+    require_cuda(weights_any, "weights");
+    TORCH_CHECK(weights_any.device() == ys.device() && weights_any.scalar_type() == at::kFloat && weights_any.numel() == p.tokens * p.k &&
+                    (weights_any.dim() == 1 ? p.k == 1 : weights_any.dim() == 2 && weights_any.size(1) == p.k),
+                "weights must be float32 [", p.tokens, ", ", p.k, "] on ", ys.device());
+    c10::cuda::CUDAGuard guard(ys.device());
+    const at::Tensor weights = weights_any.contiguous();
+    return wants_grad({&ys, &weights}) ? Combine::apply(ys, weights, position, offsets) : combine_rows(ys, weights.data_ptr<float>(), position);
+}
+
+// ---- one layer of all networks ------------------------------------------------------------------------------------------------
+
+int activation_of(c10::string_view name)
+{
+    if (name == "none") return AI2B_ACT_NONE;
+    if (name == "tanh") return AI2B_ACT_TANH;
+    if (name == "silu") return AI2B_ACT_SILU;
+    if (name == "gelu") return AI2B_ACT_GELU;
+    TORCH_CHECK(false, "activation must be none, tanh, silu or gelu (got ", name, ")");
+}
+
+ai2b_dense describe(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &offsets, int64_t activation)
+{
+    ai2b_dense d{};
+    d.dtype = dtype_of(x, "x");
+    d.activation = (int)activation;
+    d.groups = weight.dim() == 3 ? (int)weight.size(0) : 1;
+    d.inner = (int)weight.size(-1);
+    d.outer = (int)weight.size(-2);
+    d.rows = x.size(0);
+    d.d_offsets = offsets.defined() ? offsets.data_ptr<int>() : nullptr;
+    d.d_x = x.data_ptr();
+    d.x_stride = row_stride(x);
+    d.d_weight = weight.data_ptr();
+    return d;
+}
+
+// x and residual are matrices that rows_of() has passed, weight and bias contiguous. Returns y and, if they are kept, the slopes.
+std::pair<at::Tensor, at::Tensor> dense_forward(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias, const at::Tensor &residual, const at::Tensor &offsets,
+                                                int64_t activation, bool keep)
+{
+    ai2b_dense d = describe(x, weight, offsets, activation);
+    at::Tensor y = at::empty({x.size(0), d.outer}, x.options()), slope;
+    if (keep && activation != AI2B_ACT_NONE) slope = at::empty(y.sizes(), y.options().dtype(x.scalar_type() == at::kFloat ? at::kFloat : at::kHalf));
+    if (bias.defined()) d.d_bias = bias.data_ptr();
+    if (residual.defined()) {
+        d.d_residual = residual.data_ptr();
+        d.residual_stride = row_stride(residual);
+    }
+    d.d_y = y.data_ptr();
+    d.d_slope = slope.defined() ? slope.data_ptr() : nullptr;
+    const size_t bytes = ai2b_dense_workspace_bytes(&d, 0);
+    at::Tensor ws;
+    if (bytes > 0) ws = workspace(bytes, x);
+    d.d_workspace = ws.defined() ? ws.data_ptr() : nullptr;
+    d.workspace_bytes = bytes;
+    check(ai2b_dense_forward(&d, stream()), "ai2b_dense_forward");
+    return {y, slope};
+}
+
+struct Dense : torch::autograd::Function<Dense> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias_given,
+                              const std::optional<at::Tensor> &residual_given, const std::optional<at::Tensor> &offsets_given, int64_t activation)
+    {
+        const at::Tensor bias = bias_given.value_or(at::Tensor()), residual = residual_given.value_or(at::Tensor()), offsets = offsets_given.value_or(at::Tensor());
+        auto [y, slope] = dense_forward(x, weight, bias, residual, offsets, activation, x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));
+        ctx->save_for_backward({x, weight, offsets, slope});
+        ctx->saved_data["activation"] = activation;
+        const int wanted = (x.requires_grad() ? 1 : 0) | (weight.requires_grad() ? 2 : 0) | (bias.defined() && bias.requires_grad() ? 4 : 0) |
+                           (residual.defined() && residual.requires_grad() ? 8 : 0);
+        ctx->saved_data["wanted"] = (int64_t)wanted;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        require_first_order("dense");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &weight = saved[1], &offsets = saved[2], &slope = saved[3], gy = rows_of(grads[0]);
+        const int64_t wanted = ctx->saved_data["wanted"].toInt();
+        c10::cuda::CUDAGuard guard(x.device());
+        ai2b_dense d = describe(x, weight, offsets, ctx->saved_data["activation"].toInt());
+        variable_list out(6);
+        d.d_slope = slope.defined() ? slope.data_ptr() : nullptr;
+        d.d_gy = gy.data_ptr();
+        d.gy_stride = row_stride(gy);
+        if (wanted & 1) d.d_gx = (out[0] = at::empty(x.sizes(), x.options())).data_ptr();
+        if (wanted & 2) d.d_gweight = (out[1] = at::empty_like(weight)).data_ptr();
+        if (wanted & 4) d.d_gbias = (out[2] = at::empty(weight.sizes().slice(0, weight.dim() - 1), weight.options())).data_ptr();
+        if (wanted & 8) {
+            if (offsets.defined()) d.d_gresidual = (out[3] = at::empty(gy.sizes(), gy.options())).data_ptr();
+            else out[3] = grads[0];      // every row belongs to the one network
+        }
+        if (d.d_gx || d.d_gweight || d.d_gbias || d.d_gresidual) {
+            const size_t bytes = ai2b_dense_workspace_bytes(&d, 1);
+            at::Tensor ws = workspace(bytes, x);
+            d.d_workspace = ws.data_ptr();
+            d.workspace_bytes = bytes;
+            check(ai2b_dense_backward(&d, stream()), "ai2b_dense_backward");
+        }
+        return out;
+    }
+};
+
+at::Tensor dense(const at::Tensor &x_any, const at::Tensor &weight_any, const std::optional<at::Tensor> &bias_any, const std::optional<at::Tensor> &residual_any,
+                 const std::optional<at::Tensor> &offsets_any, c10::string_view activation_name)
+{
+    dtype_of(x_any, "x");
+    const int64_t activation = activation_of(activation_name);
+    require_like(weight_any, x_any, "weight");
+    const bool grouped = offsets_any.has_value();
+    TORCH_CHECK(weight_any.dim() == (grouped ? 3 : 2), grouped ? "with offsets, weight must be [groups, outer, inner]" : "without offsets, weight must be [outer, inner]",
+                " (got ", weight_any.sizes(), ")");
+    const int64_t inner = weight_any.size(-1), outer = weight_any.size(-2), groups = grouped ? weight_any.size(0) : 1;
+    TORCH_CHECK(inner >= 1 && outer >= 1 && groups >= 1 && groups <= 1024 && inner <= (1 << 20) && outer <= (1 << 20), "weight must have 1 to 1024 groups and 1 to 2^20 rows and columns (got ",
+                weight_any.sizes(), ")");
+    TORCH_CHECK(x_any.dim() >= 1 && x_any.size(-1) == inner, "the last dimension of x must be ", inner, " (got ", x_any.sizes(), ")");
+    c10::cuda::CUDAGuard guard(x_any.device());
+    const at::Tensor x = rows_of(x_any.dim() == 2 ? x_any : x_any.reshape({x_any.numel() / inner, inner})), weight = weight_any.contiguous();
+    at::Tensor bias, residual, offsets;
+    if (bias_any.has_value()) {
+        require_like(*bias_any, x_any, "bias");
+        TORCH_CHECK(bias_any->sizes() == weight.sizes().slice(0, weight.dim() - 1), "bias must be ", weight.sizes().slice(0, weight.dim() - 1), " (got ", bias_any->sizes(), ")");
+        bias = bias_any->contiguous();
+    }
+    if (residual_any.has_value()) {
+        require_like(*residual_any, x_any, "residual");
+        TORCH_CHECK(residual_any->dim() == x_any.dim() && residual_any->size(-1) == outer &&
+                        residual_any->sizes().slice(0, x_any.dim() - 1) == x_any.sizes().slice(0, x_any.dim() - 1),
+                    "residual must have the rows of x and ", outer, " columns (got ", residual_any->sizes(), ")");
+        residual = rows_of(residual_any->dim() == 2 ? *residual_any : residual_any->reshape({x.size(0), outer}));
+    }
+    if (grouped) {
+        iptr(*offsets_any, "offsets");
+        TORCH_CHECK(offsets_any->device() == x.device() && offsets_any->dim() == 1 && offsets_any->size(0) == groups + 1, "offsets must be [", groups + 1, "] on ", x.device());
+        offsets = *offsets_any;
+    }
+    at::Tensor y = wants_grad({&x, &weight, &bias, &residual}) ? Dense::apply(x, weight, given(bias), given(residual), given(offsets), activation)
+                                                               : dense_forward(x, weight, bias, residual, offsets, activation, false).first;
+    if (x_any.dim() == 2) return y;
+    auto shape = x_any.sizes().vec();
+    shape.back() = outer;
+    return y.view(shape);
+}
+
+// ---- orthogonalised updates -----------------------------------------------------------------------------------------------------
+
+at::Tensor orthogonalize(const at::Tensor &g_any, int64_t steps, double a, double b, double c, double eps)
+{
+    const int dtype = dtype_of(g_any, "g");
+    TORCH_CHECK(!wants_grad({&g_any}), "orthogonalize has no gradient: call it under torch.no_grad() or on a detached tensor");
+    TORCH_CHECK(g_any.dim() >= 2 && g_any.size(-1) >= 1 && g_any.size(-2) >= 1, "g must be [..., m, n] (got ", g_any.sizes(), ")");
+    TORCH_CHECK(steps >= 0 && steps <= 1000, "steps must be between 0 and 1000 (got ", steps, ")");
+    c10::cuda::CUDAGuard guard(g_any.device());
+    const at::Tensor g = g_any.contiguous();
+    const int64_t m = g.size(-2), n = g.size(-1), batch = g.numel() / (m * n);
+    TORCH_CHECK(batch <= 65535 && m <= (1 << 20) && n <= (1 << 20), "at most 65535 matrices of 2^20 rows and columns (got ", g.sizes(), ")");
+    at::Tensor out = at::empty_like(g);
+    const size_t bytes = ai2b_orthogonalize_workspace_bytes(dtype, (int)batch, (int)m, (int)n);
+    at::Tensor ws = workspace(bytes, g);
+    check(ai2b_orthogonalize(dtype, out.data_ptr(), g.data_ptr(), (int)batch, (int)m, (int)n, (int)steps, a, b, c, eps, ws.data_ptr(), bytes, stream()), "ai2b_orthogonalize");
+    return out;
+}
+
+}  // namespace
+
+TORCH_LIBRARY(fitnet, m)
+{
+    m.def("routeOp", &route);
+    m.def("dispatchOp", &dispatch);
+    m.def("combineOp", &combine);
+    m.def("denseOp", &dense);
+    m.def("orthogonalizeOp", &orthogonalize);
+}

@@ -1,0 +1,63 @@
+"""Fitting networks over the descriptors of this package: one network per species, or a mixture of networks per atom.
+
+    route = fitnet.route(types, ntypes)                       # atoms sorted by species (padding: negative types)
+    h = fitnet.dispatch(descriptors, route)                   # their descriptors in that order
+    h = fitnet.dense(h, w1, b1, activation="tanh", offsets=route.offsets)
+    h = fitnet.dense(h, w2, b2, residual=h, activation="tanh", offsets=route.offsets)
+    e = fitnet.combine(fitnet.dense(h, w3, b3, offsets=route.offsets), weights, route)   # back in the order of the atoms
+    update = fitnet.orthogonalize(momentum)                   # a Muon step's direction for the weight stacks
+
+The reference has per-type fitting networks in its deepmd and nn-MTP models (ai2pot/models/deepmd/se_r.py, source/descriptor/nnmtp). CUDA tensors
+only, float32, bfloat16 or float16; host tensors raise. Everything is stream-ordered, allocates through torch, never synchronises and gives the
+same bits in every call. dispatch, combine and dense are differentiable once (create_graph=True raises)."""
+import os
+from typing import NamedTuple
+
+import torch
+
+_LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libfitnet_bind.so")
+if not os.path.exists(_LIB):
+    raise ImportError(f"{_LIB} is missing: run `python -m ai2pot_b200._build` (there is no CPU fallback)")
+torch.ops.load_library(_LIB)
+
+_ops = torch.ops.fitnet
+_route, _dispatch, _combine, _dense, _orthogonalize = (op.default for op in (_ops.routeOp, _ops.dispatchOp, _ops.combineOp, _ops.denseOp, _ops.orthogonalizeOp))
+
+
+class Route(NamedTuple):
+    """Slots (entry j of token t is slot t * k + j) sorted by network. order [tokens * k]: the slots in that order, the dropped ones
+    last and as -1 - slot; position [tokens, k]: each slot's row in it, -1 if dropped; offsets [experts + 1]: first row of each network."""
+    order: torch.Tensor
+    position: torch.Tensor
+    offsets: torch.Tensor
+
+
+def route(index, experts):
+    """Sorts tokens by network (stable). index: [tokens] or [tokens, k], int32 or int64; a slot whose index is not in [0, experts) is
+    dropped. At most 1024 networks."""
+    return Route(*_route(index, experts))
+
+
+def dispatch(x, route):
+    """Rows of x [tokens, width] in the route's order: [tokens * k, width]; rows of dropped slots are zero. Differentiable in x."""
+    return _dispatch(x, *route)
+
+
+def combine(ys, weights, route):
+    """y[t] = sum over j of weights[t, j] * ys[position[t, j]] ([tokens, width]); dropped slots add nothing. weights: float32 [tokens, k].
+    Differentiable in ys and weights."""
+    return _combine(ys, weights, *route)
+
+
+def dense(x, weight, bias=None, residual=None, activation="none", offsets=None):
+    """residual + act(x @ weight.T + bias), act = none, tanh, silu or gelu (z Phi(z)). With offsets [groups + 1] (a route's), weight is
+    [groups, outer, inner], bias [groups, outer], and the rows offsets[e] to offsets[e + 1] of x belong to group e; rows after the last group
+    give zeros. Sums are float32, rounded once to the type of x. Differentiable in x, weight, bias and residual."""
+    return _dense(x, weight, bias, residual, offsets, activation)
+
+
+def orthogonalize(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """Newton-Schulz orthogonalisation of each matrix of g [..., m, n]: X = g / (|g| + eps), then `steps` times A = X X^T,
+    X = a X + (b A + c A A) X. The coefficients must keep singular values of [0, 1] bounded. No gradient."""
+    a, b, c = coefficients
+    return _orthogonalize(g, steps, a, b, c, eps)

@@ -590,6 +590,77 @@ int ai2b_evaluate(const ai2b_evaluation *e, const void *d_coords, void *stream);
  * Meant for the few kilobytes around a call, where handing over to a copy engine costs more than the copy. */
 int ai2b_chained_copy(void *dst, const void *src, size_t bytes, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Fitting networks: the pieces of per-species networks (or of a mixture of networks) over the descriptors of the calls above. The
+ * reference has per-type fitting networks in its deepmd and nn-MTP models (ai2pot/models/deepmd/se_r.py, source/descriptor/nnmtp).
+ * Element types: AI2B_F32, AI2B_BF16 or AI2B_F16 for x, weights and results of a call alike; sums are float.
+ * ---------------------------------------------------------------------------------------- */
+#define AI2B_F32 0
+#define AI2B_BF16 1
+#define AI2B_F16 2
+
+/* Rows sorted by network. Slot s = t * k + j (j < k) is entry j of token (atom) t; d_index[tokens][k] names its network, and a
+ * slot whose index is not in [0, experts) is dropped (padding).
+ *   ai2b_route                    d_order[tokens*k]: the slots sorted by network, in ascending order within one, the dropped ones
+ *                                 last and written as -1 - s; d_position[tokens][k]: the row of each slot, -1 if dropped;
+ *                                 d_offsets[experts+1]: first row of each network. At most 1024 networks, 2^31 - 1 slots.
+ *   ai2b_route_dispatch           xs[r] = x[d_order[r] / k] ([tokens*k][width]); rows of dropped slots are zero.
+ *   ai2b_route_combine            y[t] = sum_j w[t][j] ys[d_position[t][j]], added in float in the order of j; a dropped slot adds
+ *                                 nothing, whatever its weight. d_weights NULL: weights of one (the gradient of dispatch).
+ *   ai2b_route_combine_backward   gys[d_position[s]] = w[s] gy[t] (zero rows after the last network) and gw[s] = <gy[t],
+ *                                 ys[d_position[s]]> (zero for dropped slots).
+ * x, ys and gy may have row strides (in elements); outputs are contiguous and fully written. */
+size_t ai2b_route_workspace_bytes(long long tokens, int k, int experts);
+int ai2b_route(const void *d_index, int index_is_i64, long long tokens, int k, int experts,
+               int *d_order, int *d_position, int *d_offsets, void *d_workspace,
+               size_t workspace_bytes, void *stream);
+int ai2b_route_dispatch(int dtype, void *d_xs, const void *d_x, long long x_stride,
+                        const int *d_order, long long tokens, int k, int width, void *stream);
+int ai2b_route_combine(int dtype, void *d_y, const void *d_ys, long long ys_stride,
+                       const float *d_weights, const int *d_position, long long tokens, int k,
+                       int width, void *stream);
+int ai2b_route_combine_backward(int dtype, void *d_gys, float *d_gweights, const void *d_gy,
+                                long long gy_stride, const void *d_ys, long long ys_stride,
+                                const float *d_weights, const int *d_position,
+                                const int *d_offsets, long long tokens, int k, int experts,
+                                int width, void *stream);
+
+/* One layer of all networks: y = residual + act(x W_e^T + b_e) for the rows [d_offsets[e], d_offsets[e+1]) of each group e
+ * (ascending offsets from 0; NULL: one group of all rows). Rows after the last group are zero in y, gx and gresidual.
+ * The gradient call takes the slopes act'(z) that the forward call stored in d_slope (not needed without an activation).
+ * Any of d_gx, d_gweight, d_gbias, d_gresidual may be NULL. y, slope and the gradients are contiguous and fully written; every
+ * result is the same, bit for bit, in every call. Strides are in elements. At most 1024 groups. */
+#define AI2B_ACT_NONE 0
+#define AI2B_ACT_TANH 1
+#define AI2B_ACT_SILU 2
+#define AI2B_ACT_GELU 3 /* z Phi(z), the normal distribution's own Phi */
+typedef struct ai2b_dense {
+    int dtype, activation, groups, inner, outer;
+    long long rows;
+    const int *d_offsets;                                   /* [groups+1] or NULL */
+    const void *d_x;        long long x_stride;             /* [rows][inner] */
+    const void *d_weight;                                   /* [groups][outer][inner] */
+    const void *d_bias;                                     /* [groups][outer] or NULL */
+    const void *d_residual; long long residual_stride;      /* [rows][outer] or NULL */
+    void *d_y;                                              /* [rows][outer] */
+    void *d_slope;                                          /* [rows][outer], float (F32) or half (BF16, F16), or NULL: not kept */
+    const void *d_gy;       long long gy_stride;            /* [rows][outer] */
+    void *d_gx, *d_gweight, *d_gbias, *d_gresidual;
+    void *d_workspace;
+    size_t workspace_bytes;
+} ai2b_dense;
+size_t ai2b_dense_workspace_bytes(const ai2b_dense *d, int backward);
+int ai2b_dense_forward(const ai2b_dense *d, void *stream);
+int ai2b_dense_backward(const ai2b_dense *d, void *stream);
+
+/* Orthogonalised updates (as the Muon optimiser applies them to weight matrices): for each of the contiguous matrices
+ * g[batch][m][n], X = g / (|g|_F + eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X (from the right, with A = X^T X,
+ * where m > n). d_out may be d_g. */
+size_t ai2b_orthogonalize_workspace_bytes(int dtype, int batch, int m, int n);
+int ai2b_orthogonalize(int dtype, void *d_out, const void *d_g, int batch, int m, int n, int steps,
+                       double a, double b, double c, double eps, void *d_workspace,
+                       size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
