@@ -10,6 +10,7 @@
 // The sums over rows (gW, gb) are cut into slabs of rows whose partial sums are added in a fixed order: no atomics.
 #include "fitnet.cuh"
 #include "fma_tile.cuh"
+#include "matmul_tc.cuh"
 
 namespace ai2b {
 
@@ -20,18 +21,20 @@ constexpr int MAX_GROUPS = 1024;
 struct Activated {
     float value, slope;
 };
-template <int ACT>
+// QUICK: for results that are rounded to 16 bits. Exponentials and quotients of hardware precision (a few 2^-23), and the error of Phi is
+// absolute, not relative, in its lower tail: below 2^-20 of 1 + |z| in either case.
+template <int ACT, bool QUICK>
 __device__ __forceinline__ Activated activate(float z)
 {
     if constexpr (ACT == AI2B_ACT_TANH) {
-        const float t = tanhf(z);
+        const float t = QUICK ? 1.f - __fdividef(2.f, 1.f + __expf(2.f * z)) : tanhf(z);      // (an exponential that overflows gives a quotient of zero)
         return {t, 1.f - t * t};
     } else if constexpr (ACT == AI2B_ACT_SILU) {
-        const float p = 1.f / (1.f + expf(-z));
+        const float p = QUICK ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
         return {z * p, p * (1.f + z * (1.f - p))};
     } else if constexpr (ACT == AI2B_ACT_GELU) {
-        const float p = 0.5f * erfcf(-0.70710678118654752f * z);
-        return {z * p, fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), p)};
+        const float p = QUICK ? fmaf(0.5f, erff(0.70710678118654752f * z), 0.5f) : 0.5f * erfcf(-0.70710678118654752f * z);
+        return {z * p, fmaf(z * 0.39894228040143268f, QUICK ? __expf(-0.5f * z * z) : expf(-0.5f * z * z), p)};
     } else {
         return {z, 1.f};
     }
@@ -49,6 +52,10 @@ __device__ __forceinline__ long long tiles_of(long long n, int height) { return 
 // Executed by whole warps; every lane returns the same tile.
 __device__ __forceinline__ RowTile find_tile(const int *offsets, int groups, long long rows, int height, long long tile)
 {
+    if (!offsets) {
+        const long long row = tile * height;
+        return row < rows ? RowTile{0, row, min(row + height, rows)} : RowTile{-1, 0, 0};
+    }
     const int lane = threadIdx.x & 31;
     long long base = 0;
     for (int e0 = 0; e0 < groups; e0 += 32) {
@@ -72,7 +79,6 @@ __device__ __forceinline__ RowTile find_tile(const int *offsets, int groups, lon
         }
         base += __shfl_sync(FULL_MASK, scan, 31);
     }
-    if (!offsets) return RowTile{-1, 0, 0};
     const long long row = group_rows(offsets, groups - 1, rows).end + (tile - base) * height;
     if (row >= rows) return RowTile{-1, 0, 0};
     return RowTile{groups, row, min(row + height, rows)};
@@ -111,10 +117,10 @@ __device__ __forceinline__ void store_row_element(const RowOutput<T> &o, long lo
     if (o.bias) z += to_float(o.bias[(long long)group * columns + col]);
     Activated a;
     switch (o.activation) {
-    case AI2B_ACT_TANH: a = activate<AI2B_ACT_TANH>(z); break;
-    case AI2B_ACT_SILU: a = activate<AI2B_ACT_SILU>(z); break;
-    case AI2B_ACT_GELU: a = activate<AI2B_ACT_GELU>(z); break;
-    default: a = activate<AI2B_ACT_NONE>(z);
+    case AI2B_ACT_TANH: a = activate<AI2B_ACT_TANH, false>(z); break;
+    case AI2B_ACT_SILU: a = activate<AI2B_ACT_SILU, false>(z); break;
+    case AI2B_ACT_GELU: a = activate<AI2B_ACT_GELU, false>(z); break;
+    default: a = activate<AI2B_ACT_NONE, false>(z);
     }
     if (o.slope) o.slope[row * columns + col] = from_float<Slope<T>>(a.slope);
     if (o.residual) a.value += to_float(o.residual[row * o.residual_stride + col]);
@@ -170,10 +176,54 @@ __global__ void __launch_bounds__(256) weight_fma_kernel(const T *__restrict__ g
         }
 }
 
-// gz = gy * slope, gresidual = gy (zero after the last group), and the column sums of gz over each slab: part[slab][outer]
-template <typename T>
-__global__ void __launch_bounds__(256) slope_kernel(T *__restrict__ gz, T *__restrict__ gresidual, float *__restrict__ part, const T *__restrict__ gy, long long gy_stride,
-                                                    const Slope<T> *__restrict__ slope, const int *__restrict__ offsets, int groups, long long rows, int height, int outer)
+// Pieces of a float, each a bfloat16: cut off, not rounded, so that two pieces of 8 digits leave 8 for the third and their sum is the
+// float itself. What is not finite has no rest: infinities in a product of pieces give NaN.
+template <int PLANES>
+__device__ __forceinline__ void split(float v, bf16 (&out)[PLANES])
+{
+    if (!isfinite(v)) {
+        out[0] = __float2bfloat16_rn(v);
+#pragma unroll
+        for (int p = 1; p < PLANES; p++) out[p] = __float2bfloat16_rn(0.f);
+        return;
+    }
+#pragma unroll
+    for (int p = 0; p < PLANES; p++) {
+        const float piece = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+        out[p] = __float2bfloat16_rn(piece);
+        v -= piece;
+    }
+}
+
+// Operand of a tensor-core product from rows that it cannot read as they are: 16-bit rows with other alignment are copied, floats
+// are cut into PLANES planes. out[plane][row][stride], `count` rows of `columns` each.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) pack_kernel(void *__restrict__ out, long long stride, const T *__restrict__ in, long long in_stride, long long count, int columns)
+{
+    chain_wait();
+    chain_release();
+    const long long total = count * columns;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long r = i / columns;
+        const int c = (int)(i - r * columns);
+        const T v = in[r * in_stride + c];
+        if constexpr (PLANES == 1) {
+            reinterpret_cast<T *>(out)[r * stride + c] = v;
+        } else {
+            bf16 piece[PLANES];
+            split(to_float(v), piece);
+#pragma unroll
+            for (int p = 0; p < PLANES; p++) reinterpret_cast<bf16 *>(out)[(p * count + r) * stride + c] = piece[p];
+        }
+    }
+}
+
+// gz = gy * slope (as PLANES planes of pieces where that is not 1), gresidual = gy (zero after the last group), and the column sums of
+// gz over each slab: part[slab][outer]
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) slope_kernel(void *__restrict__ gz, long long gz_stride, T *__restrict__ gresidual, float *__restrict__ part, const T *__restrict__ gy,
+                                                    long long gy_stride, const Slope<T> *__restrict__ slope, const int *__restrict__ offsets, int groups, long long rows, int height,
+                                                    int outer)
 {
     __shared__ float sums[8][32];
     chain_wait();
@@ -188,9 +238,18 @@ __global__ void __launch_bounds__(256) slope_kernel(T *__restrict__ gz, T *__res
             float g = 0.f;
             if (kept) g = to_float(gy[r * gy_stride + col]);
             if (gresidual) gresidual[r * outer + col] = from_float<T>(g);
-            if (slope && kept) {
-                g *= to_float(slope[r * outer + col]);
-                gz[r * outer + col] = from_float<T>(g);
+            if (kept) {
+                if (slope) g *= to_float(slope[r * outer + col]);
+                if (gz) {
+                    if constexpr (PLANES == 1) {
+                        reinterpret_cast<T *>(gz)[r * gz_stride + col] = from_float<T>(g);
+                    } else {
+                        bf16 piece[PLANES];
+                        split(g, piece);
+#pragma unroll
+                        for (int p = 0; p < PLANES; p++) reinterpret_cast<bf16 *>(gz)[(p * rows + r) * gz_stride + col] = piece[p];
+                    }
+                }
             }
             sum += g;
         }
@@ -223,6 +282,161 @@ __global__ void __launch_bounds__(256) sum_slabs_kernel(T *__restrict__ out, con
     }
 }
 
+// ---- products on the tensor cores -------------------------------------------------------------------------------------------
+
+// Tiles of 128 rows x BN columns of one group each; the columns of a row tile follow each other, so that its rows are read from memory once
+template <int BN>
+struct RowItems {
+    const int *offsets;
+    int groups, column_tiles, inner;
+    long long rows;
+    __device__ __forceinline__ bool get(long long t, tc::Item &it) const
+    {
+        const long long m = t / column_tiles;
+        const RowTile tile = find_tile(offsets, groups, rows, tc::BM, m);
+        if (tile.group < 0) return false;
+        it.a_at = (int)tile.begin;
+        it.a_batch = 0;
+        it.b_at = it.col = (int)(t - m * column_tiles) * BN;
+        it.b_batch = tile.group;
+        it.k_begin = 0;
+        it.k_end = tile.group < groups ? inner : 0;
+        it.row = tile.begin;
+        it.row_end = tile.end;
+        it.batch = tile.group;
+        return true;
+    }
+};
+
+// bias, activation, slope and residual of 32 x 32 sums; rows of the pseudo-group are zero
+template <typename T>
+struct RowOut {
+    RowOutput<T> o;
+    int columns, groups;
+    bool vectors;             // all rows start at multiples of 16 bytes and end at whole vectors
+
+    static constexpr int N = 16 / (int)sizeof(T), LANES = 32 / N, ROWS = 32 / LANES;      // a lane takes N columns of every ROWS-th row
+    template <int ACT>
+    __device__ __forceinline__ void apply(const tc::Item &it, long long row, int col0, const float *mine, int lane) const
+    {
+        constexpr bool QUICK = sizeof(T) == 2;
+        const int i0 = lane % LANES * N, col = col0 + i0, n = min(N, columns - col);
+        if (n <= 0) return;
+        const bool kept = it.batch < groups;
+        float bias[N] = {};
+        if (o.bias && kept) {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (j < n) bias[j] = to_float(o.bias[(long long)it.batch * columns + col + j]);
+        }
+#pragma unroll 4
+        for (int r = lane / LANES; r < 32; r += ROWS) {
+            const long long at = row + r;
+            if (at >= it.row_end) return;
+            float z[N], residual[N] = {};
+            if (o.residual && kept) {
+                const T *p = o.residual + at * o.residual_stride + col;
+                if (vectors) {
+                    const Pack<T, N> v = *reinterpret_cast<const Pack<T, N> *>(p);
+#pragma unroll
+                    for (int j = 0; j < N; j++) residual[j] = to_float(v.v[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j++)
+                        if (j < n) residual[j] = to_float(p[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const float4 s = tc::staged(mine, r, (i0 + j) / 4);
+                z[j] = s.x + bias[j];
+                z[j + 1] = s.y + bias[j + 1];
+                z[j + 2] = s.z + bias[j + 2];
+                z[j + 3] = s.w + bias[j + 3];
+            }
+            Pack<T, N> y;
+            Pack<Slope<T>, N> slope;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const Activated a = kept ? activate<ACT, QUICK>(z[j]) : Activated{0.f, 0.f};
+                y.v[j] = from_float<T>(a.value + residual[j]);
+                slope.v[j] = from_float<Slope<T>>(a.slope);
+            }
+            T *py = o.out + at * columns + col;
+            Slope<T> *ps = o.slope ? o.slope + at * columns + col : nullptr;
+            if (vectors) {
+                *reinterpret_cast<Pack<T, N> *>(py) = y;
+                if (ps) *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (j < n) {
+                        py[j] = y.v[j];
+                        if (ps) ps[j] = slope.v[j];
+                    }
+            }
+        }
+    }
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col, const float *mine, int lane) const
+    {
+        switch (o.activation) {
+        case AI2B_ACT_TANH: apply<AI2B_ACT_TANH>(it, row, col, mine, lane); break;
+        case AI2B_ACT_SILU: apply<AI2B_ACT_SILU>(it, row, col, mine, lane); break;
+        case AI2B_ACT_GELU: apply<AI2B_ACT_GELU>(it, row, col, mine, lane); break;
+        default: apply<AI2B_ACT_NONE>(it, row, col, mine, lane);
+        }
+    }
+};
+
+// Tiles of gz^T x over the rows of one slab
+template <int BN>
+struct WeightItems {
+    const int *offsets;
+    int groups, height, row_tiles, column_tiles, outer;
+    long long rows;
+    __device__ __forceinline__ bool get(long long t, tc::Item &it) const
+    {
+        const int per_slab = row_tiles * column_tiles;
+        const long long slab = t / per_slab;
+        const RowTile tile = find_tile(offsets, groups, rows, height, slab);
+        if (tile.group < 0 || tile.group >= groups) return false;
+        const int i = (int)(t - slab * per_slab);
+        it.a_at = i / column_tiles * tc::BM;
+        it.b_at = it.col = i % column_tiles * BN;
+        it.a_batch = it.b_batch = 0;
+        it.k_begin = (int)tile.begin;
+        it.k_end = (int)tile.end;
+        it.row = it.a_at;
+        it.row_end = outer;
+        it.batch = (int)slab;
+        return true;
+    }
+};
+struct WeightOut {
+    float *part;              // [slab][outer][inner]
+    int columns, outer;
+    bool vectors;
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane) const
+    {
+        const int i = lane & 7, col = col0 + 4 * i;
+        if (col >= columns) return;
+#pragma unroll
+        for (int r = lane >> 3; r < 32; r += 4) {
+            if (row + r >= it.row_end) return;
+            const float4 v = tc::staged(mine, r, i);
+            float *p = part + ((long long)it.batch * outer + row + r) * columns + col;
+            if (vectors) {
+                *reinterpret_cast<float4 *>(p) = v;
+            } else {
+                p[0] = v.x;
+                if (col + 1 < columns) p[1] = v.y;
+                if (col + 2 < columns) p[2] = v.z;
+                if (col + 3 < columns) p[3] = v.w;
+            }
+        }
+    }
+};
+
 // ---- host side ------------------------------------------------------------------------------------------------------------
 
 // Rows of a slab: enough slabs that the products of a slab keep all SMs busy, none shorter than 256 rows
@@ -236,25 +450,158 @@ static int slab_height(long long rows, long long tiles_per_slab)
 }
 static long long slab_bound(long long rows, int height, int groups) { return (rows + height - 1) / height + groups; }
 
-struct BackwardPlan {
-    int weight_height, bias_height;
-    size_t gz, weight_part, bias_part, total;
+static int planes_of(int dtype) { return dtype == AI2B_F32 ? 3 : 1; }
+static long long padded(long long n) { return (n + 7) / 8 * 8; }
+
+// The FMA pipes take what is small: there the tensor-core kernel's set-up (barriers, TMEM, tensor maps) is not made up for.
+static bool on_tensor_cores(const ai2b_dense *d) { return d->rows > 0 && (double)d->rows * d->inner * d->outer >= 4e6; }
+
+// An operand of a tensor-core product: rows as they lie in memory, or a packed copy of them in the workspace
+struct PackedRows {
+    const void *from;
+    long long from_stride, count, columns;
+    bool copy;
+    size_t at;                // of the copy in the workspace
+    long long stride() const { return copy ? padded(columns) : from_stride; }
 };
+static PackedRows packed_rows(int dtype, const void *from, long long stride, long long count, long long columns, size_t *at)
+{
+    PackedRows p{from, stride, count, columns, false, *at};
+    p.copy = dtype == AI2B_F32 || common_alignment(from, stride * 2) < 16;
+    if (p.copy) *at += round256(2 * (size_t)planes_of(dtype) * count * padded(columns));
+    return p;
+}
+
+struct ForwardPlan {
+    bool tensor;
+    PackedRows x, weight;
+    size_t total;
+};
+static ForwardPlan plan_forward(const ai2b_dense *d)
+{
+    ForwardPlan p{};
+    p.tensor = on_tensor_cores(d);
+    if (p.tensor) {
+        p.x = packed_rows(d->dtype, d->d_x, d->x_stride, d->rows, d->inner, &p.total);
+        p.weight = packed_rows(d->dtype, d->d_weight, d->inner, (long long)d->groups * d->outer, d->inner, &p.total);
+    }
+    return p;
+}
+
+struct BackwardPlan {
+    bool tensor, slopes;
+    int weight_height, bias_height;
+    PackedRows gz, x, weight;     // gz.copy: made by slope_kernel
+    size_t weight_part, bias_part, total;
+};
+static int columns_of_tile(int dtype, int columns);
 static BackwardPlan plan_backward(const ai2b_dense *d)
 {
     BackwardPlan p{};
-    const long long tiles = (long long)((d->outer + FT - 1) / FT) * ((d->inner + FT - 1) / FT);
-    p.weight_height = slab_height(d->rows, tiles);
+    p.tensor = on_tensor_cores(d);
+    p.slopes = d->activation != AI2B_ACT_NONE;
+    const int bm = p.tensor ? tc::BM : FT, bn = p.tensor ? columns_of_tile(d->dtype, d->inner) : FT;
+    p.weight_height = slab_height(d->rows, (long long)((d->outer + bm - 1) / bm) * ((d->inner + bn - 1) / bn));
     p.bias_height = slab_height(d->rows, (d->outer + 31) / 32);
-    size_t at = 0;
-    p.gz = at;
-    if (d->activation != AI2B_ACT_NONE) at += round256(element_bytes(d->dtype) * (size_t)d->rows * d->outer);
-    p.weight_part = at;
-    at += round256(sizeof(float) * (size_t)slab_bound(d->rows, p.weight_height, d->groups) * d->outer * d->inner);
-    p.bias_part = at;
-    at += round256(sizeof(float) * (size_t)slab_bound(d->rows, p.bias_height, d->groups) * d->outer);
-    p.total = at;
+    if (p.tensor) {
+        p.gz = packed_rows(d->dtype, p.slopes ? nullptr : d->d_gy, p.slopes ? 1 : d->gy_stride, d->rows, d->outer, &p.total);
+        p.x = packed_rows(d->dtype, d->d_x, d->x_stride, d->rows, d->inner, &p.total);
+        p.weight = packed_rows(d->dtype, d->d_weight, d->inner, (long long)d->groups * d->outer, d->inner, &p.total);
+    } else {
+        p.gz = PackedRows{d->d_gy, d->gy_stride, d->rows, d->outer, false, 0};
+        if (p.slopes) {
+            p.gz.copy = true;
+            p.total += round256(element_bytes(d->dtype) * (size_t)d->rows * padded(d->outer));
+        }
+    }
+    p.weight_part = p.total;
+    p.total += round256(sizeof(float) * (size_t)slab_bound(d->rows, p.weight_height, d->groups) * d->outer * d->inner);
+    p.bias_part = p.total;
+    p.total += round256(sizeof(float) * (size_t)slab_bound(d->rows, p.bias_height, d->groups) * d->outer);
     return p;
+}
+
+template <typename T>
+static int pack(const PackedRows &p, unsigned char *ws, cudaStream_t st)
+{
+    if (!p.copy) return AI2B_OK;
+    const long long blocks = (p.count * p.columns + 255) / 256;
+    constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
+    AI2B_CUDA(launch_chained(pack_kernel<T, PLANES>, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st, (void *)(ws + p.at), p.stride(), (const T *)p.from,
+                             p.from_stride, p.count, (int)p.columns));
+    return AI2B_OK;
+}
+
+// Tensor map of `batch` matrices of `rows` rows each (and their further planes)
+static int map_rows(CUtensorMap *map, int dtype, const PackedRows &p, const unsigned char *ws, long long rows, long long batch, int box_rows)
+{
+    return tc::make_map(map, p.copy ? ws + p.at : p.from, dtype != AI2B_F16, p.columns, rows, batch * planes_of(dtype), p.stride(), rows * p.stride(), box_rows);
+}
+
+// Columns of a tile: the width that wastes the fewest columns, and the wider of two that waste as many. Three planes of 256 columns do not
+// fit two stages.
+static int columns_of_tile(int dtype, int columns)
+{
+    int best = 64;
+    for (int bn = 128; bn <= (dtype == AI2B_F32 ? 128 : 256); bn *= 2)
+        if ((columns + bn - 1) / bn * bn <= (columns + best - 1) / best * best) best = bn;
+    return best;
+}
+
+// f(integral_constant<BN>)
+template <typename T, typename F>
+static int with_columns(int bn, F &&f)
+{
+    if (bn == 64) return f(std::integral_constant<int, 64>{});
+    if constexpr (sizeof(T) == 2)
+        if (bn == 256) return f(std::integral_constant<int, 256>{});
+    return f(std::integral_constant<int, 128>{});
+}
+
+template <typename T>
+static bool rows_in_vectors(const RowOutput<T> &o, int columns)
+{
+    return common_alignment(o.out, o.slope, o.residual, (long long)sizeof(T) * columns, o.residual ? (long long)sizeof(T) * o.residual_stride : 0LL) >= 16;
+}
+
+// rows times the matrices of their groups: B_MN = false for x W^T, true for gz W
+template <typename T, bool B_MN>
+static int multiply_rows(const ai2b_dense *d, const PackedRows &a, const PackedRows &w, const unsigned char *ws, const RowOutput<T> &o, int inner, int columns, cudaStream_t st)
+{
+    constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
+    return with_columns<T>(columns_of_tile(d->dtype, columns), [&](auto bn) {
+        constexpr int BN = decltype(bn)::value;
+        tc::Operands ops{};
+        int rc = map_rows(&ops.a, d->dtype, a, ws, d->rows, 1, tc::BM);
+        if (rc == AI2B_OK) rc = map_rows(&ops.b, d->dtype, w, ws, d->outer, d->groups, B_MN ? 64 : BN);
+        if (rc == AI2B_OK) rc = tc::flag_address(&ops.gave_up);
+        if (rc != AI2B_OK) return rc;
+        ops.a_stack = 1;
+        ops.b_stack = d->groups;
+        ops.is_bf16 = d->dtype != AI2B_F16;
+        const RowItems<BN> items{d->d_offsets, d->groups, (columns + BN - 1) / BN, inner, d->rows};
+        const RowOut<T> out{o, columns, d->groups, rows_in_vectors(o, columns)};
+        return tc::launch<PLANES, BN, false, B_MN>(ops, items, out, ((d->rows + tc::BM - 1) / tc::BM + d->groups) * items.column_tiles, st);
+    });
+}
+
+template <typename T>
+static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const unsigned char *ws, float *part, cudaStream_t st)
+{
+    constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
+    return with_columns<T>(columns_of_tile(d->dtype, d->inner), [&](auto bn) {
+        constexpr int BN = decltype(bn)::value;
+        tc::Operands ops{};
+        int rc = map_rows(&ops.a, d->dtype, p.gz, ws, d->rows, 1, 64);
+        if (rc == AI2B_OK) rc = map_rows(&ops.b, d->dtype, p.x, ws, d->rows, 1, 64);
+        if (rc == AI2B_OK) rc = tc::flag_address(&ops.gave_up);
+        if (rc != AI2B_OK) return rc;
+        ops.a_stack = ops.b_stack = 1;
+        ops.is_bf16 = d->dtype != AI2B_F16;
+        const WeightItems<BN> items{d->d_offsets, d->groups, p.weight_height, (d->outer + tc::BM - 1) / tc::BM, (d->inner + BN - 1) / BN, d->outer, d->rows};
+        const WeightOut out{part, d->inner, d->outer, d->inner % 4 == 0};
+        return tc::launch<PLANES, BN, true, true>(ops, items, out, slab_bound(d->rows, p.weight_height, d->groups) * items.row_tiles * items.column_tiles, st);
+    });
 }
 
 static int check_dense(const ai2b_dense *d, const char *what)
@@ -280,8 +627,8 @@ using namespace ai2b;
 
 extern "C" size_t ai2b_dense_workspace_bytes(const ai2b_dense *d, int backward)
 {
-    if (!d || check_dense(d, "ai2b_dense_workspace_bytes") != AI2B_OK || !backward) return 256;
-    return plan_backward(d).total + 256;
+    if (!d || check_dense(d, "ai2b_dense_workspace_bytes") != AI2B_OK) return 0;
+    return backward ? plan_backward(d).total : plan_forward(d).total;
 }
 
 extern "C" int ai2b_dense_forward(const ai2b_dense *d, void *stream)
@@ -291,11 +638,21 @@ extern "C" int ai2b_dense_forward(const ai2b_dense *d, void *stream)
     AI2B_REQUIRE(d->d_y, AI2B_ERR_INVALID, "ai2b_dense_forward: y is NULL");
     AI2B_REQUIRE(!d->d_residual || d->residual_stride >= d->outer || d->rows == 1, AI2B_ERR_INVALID, "ai2b_dense_forward: row stride %lld of the residual is below %d",
                  d->residual_stride, d->outer);
+    const ForwardPlan p = plan_forward(d);
+    AI2B_REQUIRE(p.total == 0 || (d->d_workspace && d->workspace_bytes >= p.total), AI2B_ERR_WORKSPACE, "ai2b_dense_forward: workspace of %zu bytes, %zu needed",
+                 d->workspace_bytes, p.total);
     cudaStream_t st = (cudaStream_t)stream;
+    unsigned char *ws = (unsigned char *)d->d_workspace;
     return with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
         const RowOutput<T> o{(T *)d->d_y, d->activation != AI2B_ACT_NONE ? (Slope<T> *)d->d_slope : nullptr, (const T *)d->d_bias, (const T *)d->d_residual, d->residual_stride,
                              d->activation};
+        if (p.tensor) {
+            int rc2 = pack<T>(p.x, ws, st);
+            if (rc2 == AI2B_OK) rc2 = pack<T>(p.weight, ws, st);
+            if (rc2 == AI2B_OK) rc2 = multiply_rows<T, false>(d, p.x, p.weight, ws, o, d->inner, d->outer, st);
+            return rc2;
+        }
         const dim3 grid((unsigned)((d->rows + FT - 1) / FT + d->groups), (d->outer + FT - 1) / FT);
         AI2B_CUDA(launch_chained(rows_fma_kernel<T>, grid, dim3(256), 0, st, (const T *)d->d_x, d->x_stride, (const T *)d->d_weight, (long long)d->outer * d->inner,
                                  (long long)d->inner, 1LL, d->d_offsets, d->groups, d->rows, d->inner, d->outer, o));
@@ -317,31 +674,45 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
     unsigned char *ws = (unsigned char *)d->d_workspace;
     return with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
-        T *made = (T *)(ws + p.gz);
-        const T *gz = slopes ? made : (const T *)d->d_gy;
-        const long long gz_stride = slopes ? d->outer : d->gy_stride;
+        const bool products = d->rows > 0 && (d->d_gx || d->d_gweight), make_gz = products && p.gz.copy;
         float *wpart = (float *)(ws + p.weight_part), *bpart = (float *)(ws + p.bias_part);
-        const bool products = d->d_gx || d->d_gweight;
-        if (d->rows > 0 && ((slopes && products) || d->d_gresidual || d->d_gbias)) {
+        if (d->rows > 0 && (make_gz || d->d_gresidual || d->d_gbias)) {
             const dim3 grid((unsigned)(slab_bound(d->rows, p.bias_height, d->groups) + 1), (d->outer + 31) / 32);
-            AI2B_CUDA(launch_chained(slope_kernel<T>, grid, dim3(256), 0, st, made, (T *)d->d_gresidual, d->d_gbias ? bpart : (float *)nullptr, (const T *)d->d_gy,
-                                     d->gy_stride, slopes ? (const Slope<T> *)d->d_slope : (const Slope<T> *)nullptr, d->d_offsets, d->groups, d->rows, p.bias_height, d->outer));
+            auto go = [&](auto kern) {
+                return launch_chained(kern, grid, dim3(256), 0, st, make_gz ? (void *)(ws + p.gz.at) : (void *)nullptr, p.gz.stride(), (T *)d->d_gresidual,
+                                      d->d_gbias ? bpart : (float *)nullptr, (const T *)d->d_gy, d->gy_stride,
+                                      slopes ? (const Slope<T> *)d->d_slope : (const Slope<T> *)nullptr, d->d_offsets, d->groups, d->rows, p.bias_height, d->outer);
+            };
+            if constexpr (std::is_same<T, float>::value)
+                if (p.tensor) AI2B_CUDA(go(slope_kernel<float, 3>));
+            if (!(std::is_same<T, float>::value && p.tensor)) AI2B_CUDA(go(slope_kernel<T, 1>));
         }
         if (d->d_gbias) {
             const dim3 grid((d->outer + 255) / 256, d->groups);
             AI2B_CUDA(launch_chained(sum_slabs_kernel<T>, grid, dim3(256), 0, st, (T *)d->d_gbias, (const float *)bpart, d->d_offsets, d->rows, p.bias_height,
                                      (long long)d->outer, slab_bound(d->rows, p.bias_height, d->groups)));
         }
+        const T *gz = (const T *)(p.gz.copy ? ws + p.gz.at : d->d_gy);
         if (d->d_gx && d->rows > 0) {
             const RowOutput<T> o{(T *)d->d_gx, nullptr, nullptr, nullptr, 0, AI2B_ACT_NONE};
-            const dim3 grid((unsigned)((d->rows + FT - 1) / FT + d->groups), (d->inner + FT - 1) / FT);
-            AI2B_CUDA(launch_chained(rows_fma_kernel<T>, grid, dim3(256), 0, st, gz, gz_stride, (const T *)d->d_weight, (long long)d->outer * d->inner, 1LL,
-                                     (long long)d->inner, d->d_offsets, d->groups, d->rows, d->outer, d->inner, o));
+            if (p.tensor) {
+                int rc2 = pack<T>(p.weight, ws, st);
+                if (rc2 == AI2B_OK) rc2 = multiply_rows<T, true>(d, p.gz, p.weight, ws, o, d->outer, d->inner, st);
+                if (rc2 != AI2B_OK) return rc2;
+            } else {
+                const dim3 grid((unsigned)((d->rows + FT - 1) / FT + d->groups), (d->inner + FT - 1) / FT);
+                AI2B_CUDA(launch_chained(rows_fma_kernel<T>, grid, dim3(256), 0, st, gz, p.gz.stride(), (const T *)d->d_weight, (long long)d->outer * d->inner, 1LL,
+                                         (long long)d->inner, d->d_offsets, d->groups, d->rows, d->outer, d->inner, o));
+            }
         }
         if (d->d_gweight) {
-            if (d->rows > 0) {
+            if (p.tensor) {
+                int rc2 = pack<T>(p.x, ws, st);
+                if (rc2 == AI2B_OK) rc2 = multiply_weight<T>(d, p, ws, wpart, st);
+                if (rc2 != AI2B_OK) return rc2;
+            } else if (d->rows > 0) {
                 const dim3 grid((unsigned)slab_bound(d->rows, p.weight_height, d->groups), (d->outer + FT - 1) / FT, (d->inner + FT - 1) / FT);
-                AI2B_CUDA(launch_chained(weight_fma_kernel<T>, grid, dim3(256), 0, st, gz, gz_stride, (const T *)d->d_x, d->x_stride, d->d_offsets, d->groups, d->rows,
+                AI2B_CUDA(launch_chained(weight_fma_kernel<T>, grid, dim3(256), 0, st, gz, p.gz.stride(), (const T *)d->d_x, d->x_stride, d->d_offsets, d->groups, d->rows,
                                          p.weight_height, d->outer, d->inner, wpart));
             }
             const long long size = (long long)d->outer * d->inner;

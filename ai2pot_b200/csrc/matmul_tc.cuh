@@ -1,0 +1,334 @@
+// Matrix products on the fifth-generation tensor cores, for the fitting-network kernels.
+//
+// One persistent block per SM. A producer warp copies operand tiles to shared memory with TMA, one thread of a second warp issues
+// tcgen05.mma into one of two accumulators in TMEM, eight warps take finished accumulators out and hand them to an epilogue while
+// the next tile is being multiplied. Tiles are 128 x BN, 64 of the summed index per stage.
+//
+// Operands are 16-bit matrices in memory with 16-byte aligned rows, read in the direction that they lie in: an operand whose rows run
+// along the summed index is K-major, one whose rows run along the tile's own index is MN-major (the tensor core takes both), so no
+// operand is transposed.
+//
+// More digits than 16 bits hold come in planes: a matrix as a sum of PLANES 16-bit matrices, hi + mid (+ lo), each a further piece of the
+// significand. The product is the sum of the plane products of order below PLANES (1, 3 or 6 of them), added up in the same float accumulator;
+// a stage holds all planes of its tiles, so each is loaded once.
+//
+// Every wait ends: after WAIT_LIMIT tries a role gives up, the block waits (bounded again) for its copies and products in flight, frees its
+// TMEM, raises a flag that ai2b_fitnet_check() reports, and returns.
+#pragma once
+#include <cuda.h>
+#include "fitnet.cuh"
+
+namespace ai2b {
+namespace tc {
+
+constexpr int BM = 128, BK = 64;
+constexpr int EPILOGUE_WARPS = 8, THREADS = 64 + 32 * EPILOGUE_WARPS;
+constexpr int STAGE_LIMIT = 8;
+constexpr int STAGING_BYTES = EPILOGUE_WARPS * 32 * 32 * 4;      // per epilogue warp 32 rows x 32 columns of float
+constexpr int SMEM_BUDGET = 227 * 1024;
+constexpr int WAIT_LIMIT = 1 << 22;
+
+// ---- PTX ------------------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void barrier_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void barrier_expect(unsigned bar, unsigned bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool barrier_try(unsigned bar, unsigned parity)
+{
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool barrier_wait(unsigned bar, unsigned parity)
+{
+    bool ok = false;
+    for (int i = 0; i < WAIT_LIMIT && !ok; i++) ok = barrier_try(bar, parity);
+    return __all_sync(FULL_MASK, ok);      // whole warps wait, and go on or give up together
+}
+
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, int x, int y, int z, unsigned bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z),
+                 "r"(bar)
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"((unsigned)accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void commit(unsigned bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(float (&v)[32], unsigned addr)
+{
+    unsigned *r = reinterpret_cast<unsigned *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+        "%26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+
+// Shared-memory matrix descriptor of a tile of rows of 128 bytes with the 128-byte swizzle. leading: bytes between neighbouring
+// 64-element columns of an MN-major tile (not used for a K-major one); groups of eight rows follow each other without gaps.
+__device__ __forceinline__ unsigned long long tile_descriptor(unsigned address, unsigned leading)
+{
+    return (unsigned long long)((address >> 4) & 0x3fff) | (unsigned long long)((leading >> 4) & 0x3fff) << 16 | (unsigned long long)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// Instruction descriptor: float accumulator, operands both bfloat16 or both half
+__host__ __device__ constexpr unsigned instruction_descriptor(bool is_bf16, bool a_mn, bool b_mn, int n)
+{
+    return 1u << 4 | (is_bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (unsigned)(n >> 3) << 17 | (unsigned)(BM >> 4) << 24;
+}
+
+// ---- a tile of work -------------------------------------------------------------------------------------------------------
+
+struct Item {
+    int a_at, b_at;               // first row of the tile in each operand's own index
+    int a_batch, b_batch;         // matrix (of the first plane) in the operand's stack; planes follow each other a stack further on
+    int k_begin, k_end;           // range of the summed index; k_begin == k_end: the sums are zero
+    long long row, row_end;       // rows and first column of the result
+    int col, batch;
+};
+
+template <int PLANES, int BN>
+struct Shape {
+    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;      // one plane
+    static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
+    static constexpr int STAGES_FIT = (SMEM_BUDGET - STAGING_BYTES - 2048) / STAGE_BYTES;
+    static constexpr int STAGES = STAGES_FIT < STAGE_LIMIT ? STAGES_FIT : STAGE_LIMIT;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + STAGING_BYTES + 2048;      // with 1024 bytes to align by and 1024 for barriers
+    static_assert(STAGES >= 2, "two stages at least");
+};
+
+// A plane's tile in a stage: K-major one box of 64 x rows, MN-major a box of 64 x 64 for every 64 rows of the tile
+template <bool MN>
+__device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap *map, int rows, int at, int k, int batch, unsigned bar)
+{
+    if constexpr (MN) {
+        for (int c = 0; c < rows; c += 64) tma_load(dst + c * BK * 2, map, at + c, k, batch, bar);
+    } else {
+        tma_load(dst, map, k, at, batch, bar);
+    }
+}
+
+struct Operands {
+    CUtensorMap a, b;
+    int a_stack, b_stack;         // matrices in one plane of each operand
+    int is_bf16;
+    int *gave_up;                 // set by a wait that ran out
+};
+
+// Tiles: Items::get(long long t, Item &) by whole warps, false after the last one. Out: out(item, lane quarter's row, column, accumulators).
+template <int PLANES, int BN, bool A_MN, bool B_MN, typename Items, typename Out>
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Operands ops, const __grid_constant__ Items items, const __grid_constant__ Out out)
+{
+    using S = Shape<PLANES, BN>;
+    extern __shared__ unsigned char smem_raw[];
+    const unsigned raw = smem_address(smem_raw), base = (raw + 1023) & ~1023u;
+    unsigned char *smem = smem_raw + (base - raw);
+    float *staging = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE_BYTES);
+    const unsigned bars = base + S::STAGES * S::STAGE_BYTES + STAGING_BYTES;
+    const unsigned full = bars, empty = bars + 8 * STAGE_LIMIT, done = empty + 8 * STAGE_LIMIT, taken = done + 16, drained = taken + 16;
+    unsigned *tmem_slot = reinterpret_cast<unsigned *>(smem + (drained + 8 - base));
+    int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int TMEM_COLUMNS = 2 * BN;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; s++) {
+            barrier_init(full + 8 * s, 1);
+            barrier_init(empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            barrier_init(done + 8 * b, 1);
+            barrier_init(taken + 8 * b, EPILOGUE_WARPS);
+        }
+        barrier_init(drained, 1);
+        *stopped = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(TMEM_COLUMNS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = *tmem_slot;
+    chain_wait();
+    chain_release();
+
+    bool ok = true;
+    unsigned issued = 0;                 // stages that the producer has started
+    if (warp == 0) {
+        Item it;
+        for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
+            for (int k = it.k_begin; ok && k < it.k_end; k += BK, issued++) {
+                const unsigned s = issued % S::STAGES, round = issued / S::STAGES;
+                ok = round == 0 || barrier_wait(empty + 8 * s, (round - 1) & 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    barrier_expect(full + 8 * s, S::STAGE_BYTES);
+                    const unsigned dst = base + s * S::STAGE_BYTES;
+#pragma unroll
+                    for (int p = 0; p < PLANES; p++) {
+                        load_tile<A_MN>(dst + p * S::A_BYTES, &ops.a, BM, it.a_at, k, it.a_batch + p * ops.a_stack, full + 8 * s);
+                        load_tile<B_MN>(dst + PLANES * S::A_BYTES + p * S::B_BYTES, &ops.b, BN, it.b_at, k, it.b_batch + p * ops.b_stack, full + 8 * s);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 1) {
+        const unsigned idesc = instruction_descriptor(ops.is_bf16, A_MN, B_MN, BN);
+        Item it;
+        unsigned used = 0, tile = 0;
+        for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
+            if (it.k_begin >= it.k_end) continue;
+            const unsigned buf = tile & 1, d = tmem + buf * BN;
+            if (tile >= 2) ok = barrier_wait(taken + 8 * buf, ((tile >> 1) - 1) & 1);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int k = it.k_begin; k < it.k_end; k += BK, used++) {
+                const unsigned s = used % S::STAGES;
+                ok = barrier_wait(full + 8 * s, (used / S::STAGES) & 1);
+                if (!ok) break;
+                const unsigned a = base + s * S::STAGE_BYTES, b = a + PLANES * S::A_BYTES;
+                const int left = it.k_end - k, steps = left >= BK ? BK / 16 : (left + 15) / 16;
+                if constexpr (A_MN && B_MN) {
+                    // The summed index runs over rows of memory, and what follows k_end may belong to another network: it may hold NaN, so it
+                    // is zeroed in both operands up to the 16 rows of the last step. A row is 128 whole bytes whatever the swizzle.
+                    if (left < steps * 16) {
+                        for (int i = lane; i < (steps * 16 - left) * 8; i += 32) {
+                            const unsigned at = (left + (i >> 3)) * 128 + (i & 7) * 16;
+                            for (int c = 0; c < PLANES * (BM + BN) / 64; c++)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a + c * BK * 128 + at), "r"(0) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (lane == 0) {
+                    for (int step = 0; step < steps; step++) {
+                        // 16 of the summed index: 32 bytes along a K-major row, 16 rows of an MN-major tile
+                        const unsigned a_step = step * (A_MN ? 16 * 128 : 32), b_step = step * (B_MN ? 16 * 128 : 32);
+                        bool more = k > it.k_begin || step > 0;
+#pragma unroll
+                        for (int order = PLANES - 1; order >= 0; order--) {      // small pieces first
+#pragma unroll
+                            for (int pa = 0; pa <= order; pa++) {
+                                mma(d, tile_descriptor(a + pa * S::A_BYTES + a_step, BK * 128), tile_descriptor(b + (order - pa) * S::B_BYTES + b_step, BK * 128), idesc, more);
+                                more = true;
+                            }
+                        }
+                    }
+                    commit(empty + 8 * s);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (lane == 0) commit(done + 8 * buf);
+            __syncwarp();
+            tile++;
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        float *mine = staging + (warp - 2) * 1024;
+        Item it;
+        unsigned tile = 0;
+        for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
+            const bool sums = it.k_begin < it.k_end;
+            const unsigned buf = tile & 1;
+            if (sums) {
+                ok = barrier_wait(done + 8 * buf, (tile >> 1) & 1);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            const long long row = it.row + 32 * quarter;
+            for (int c = 32 * half; c < BN; c += 64) {
+                if (row >= it.row_end || it.col + c >= out.columns) break;
+                float v[32];
+                if (sums) {
+                    tmem_load32(v, tmem + buf * BN + c + ((unsigned)(32 * quarter) << 16));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = 0.f;
+                }
+                // Lane l holds row l: through shared memory, so that neighbouring lanes get neighbouring columns. Four columns at a time,
+                // permuted within the row, keep both directions free of bank conflicts.
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    *reinterpret_cast<float4 *>(mine + 32 * lane + 4 * (i ^ (lane & 7))) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                __syncwarp();
+                out(it, row, it.col + c, mine, lane);
+                __syncwarp();
+            }
+            if (sums) {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                if (lane == 0) barrier_arrive(taken + 8 * buf);
+                tile++;
+            }
+        }
+    }
+    if (!ok && lane == 0) {
+        *stopped = 1;
+        *ops.gave_up = 1;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (*stopped) {
+        // copies in flight write into this block's shared memory, products into its TMEM
+        if (warp == 0)
+            for (unsigned i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; i++) barrier_wait(full + 8 * (i % S::STAGES), (i / S::STAGES) & 1);
+        if (warp == 1) {
+            if (lane == 0) commit(drained);
+            barrier_wait(drained, 0);
+        }
+        __syncthreads();
+    }
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS) : "memory");
+}
+
+// What an epilogue reads of a warp's 32 x 32 sums: columns [4 i, 4 i + 4) of row r
+__device__ __forceinline__ float4 staged(const float *mine, int r, int i) { return *reinterpret_cast<const float4 *>(mine + 32 * r + 4 * (i ^ (r & 7))); }
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+
+// Tensor map of matrices [batch][rows][columns] with 16-bit elements: boxes of 64 columns x box_rows rows, 128-byte swizzle; what lies
+// outside the matrix reads as zero. The address and the strides in bytes are multiples of 16.
+// flag_address: where the current device's products report a wait that ran out
+int flag_address(int **flag);
+int make_map(CUtensorMap *map, const void *p, bool is_bf16, long long columns, long long rows, long long batch, long long row_stride, long long batch_stride, int box_rows);
+
+template <int PLANES, int BN, bool A_MN, bool B_MN, typename Items, typename Out>
+int launch(const Operands &ops, const Items &items, const Out &out, long long tiles, cudaStream_t st)
+{
+    using S = Shape<PLANES, BN>;
+    auto kern = product_kernel<PLANES, BN, A_MN, B_MN, Items, Out>;
+    static KernelSetup ks;
+    const int rc = kernel_setup(ks, kern, S::SMEM);
+    if (rc != AI2B_OK) return rc;
+    const int sms = sm_count();
+    AI2B_CUDA(launch_chained(kern, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(THREADS), S::SMEM, st, ops, items, out));
+    return AI2B_OK;
+}
+
+}  // namespace tc
+}  // namespace ai2b

@@ -15,6 +15,8 @@ from typing import NamedTuple
 
 import torch
 
+from . import capi
+
 _LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libfitnet_bind.so")
 if not os.path.exists(_LIB):
     raise ImportError(f"{_LIB} is missing: run `python -m ai2pot_b200._build` (there is no CPU fallback)")
@@ -61,3 +63,9 @@ def orthogonalize(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     X = a X + (b A + c A A) X. The coefficients must keep singular values of [0, 1] bounded. No gradient."""
     a, b, c = coefficients
     return _orthogonalize(g, steps, a, b, c, eps)
+
+
+def check():
+    """Waits for the current stream and raises if a tensor-core product of this device has given up waiting for its own copies since the
+    last check. (Every wait of the kernels is bounded; none should run out.)"""
+    capi._check(capi.lib().ai2b_fitnet_check(capi._stream()))

@@ -649,9 +649,15 @@ typedef struct ai2b_dense {
     void *d_workspace;
     size_t workspace_bytes;
 } ai2b_dense;
+/* Scratch of the forward (0) or gradient (1) call of this description, whose pointers, strides and sizes have to be set: operands
+ * that are not aligned to 16 bytes, and float ones, are laid out there for the tensor cores. */
 size_t ai2b_dense_workspace_bytes(const ai2b_dense *d, int backward);
 int ai2b_dense_forward(const ai2b_dense *d, void *stream);
 int ai2b_dense_backward(const ai2b_dense *d, void *stream);
+
+/* AI2B_ERR_TIMEOUT if a tensor-core product of this device has given up waiting for its own copies since the last check (every wait is
+ * bounded; none should run out), AI2B_OK otherwise. Synchronises the stream. */
+int ai2b_fitnet_check(void *stream);
 
 /* Orthogonalised updates (as the Muon optimiser applies them to weight matrices): for each of the contiguous matrices
  * g[batch][m][n], X = g / (|g|_F + eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X (from the right, with A = X^T X,

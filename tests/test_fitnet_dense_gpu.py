@@ -9,6 +9,12 @@ pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
     from ai2pot_b200 import fitnet
 
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    fitnet.check()
+
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 

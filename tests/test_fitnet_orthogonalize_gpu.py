@@ -13,6 +13,12 @@ pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
     from ai2pot_b200 import fitnet
 
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    fitnet.check()
+
 MUON = (3.4445, -4.7750, 2.0315)
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
