@@ -219,66 +219,120 @@ __global__ void __launch_bounds__(256) pack_kernel(void *__restrict__ out, long 
 }
 
 // gz = gy * slope (as PLANES planes of pieces where that is not 1), gresidual = gy (zero after the last group), and the column sums of
-// gz over each slab: part[slab][outer]
-template <typename T, int PLANES>
+// gz over each slab: part[slab][outer]. A lane takes N columns, a warp every eighth row of the slab, four of them in flight.
+template <typename T, int PLANES, int N>
 __global__ void __launch_bounds__(256) slope_kernel(void *__restrict__ gz, long long gz_stride, T *__restrict__ gresidual, float *__restrict__ part, const T *__restrict__ gy,
                                                     long long gy_stride, const Slope<T> *__restrict__ slope, const int *__restrict__ offsets, int groups, long long rows, int height,
                                                     int outer)
 {
-    __shared__ float sums[8][32];
+    __shared__ float sums[8][32 * N];
     chain_wait();
     chain_release();
     const RowTile tile = find_tile(offsets, groups, rows, height, blockIdx.x);
     if (tile.group < 0) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * 32 + lane;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.y * 32 + lane) * N;
     const bool kept = tile.group < groups;
-    float sum = 0.f;
+    float sum[N] = {};
     if (col < outer) {
-        for (long long r = tile.begin + warp; r < tile.end; r += 8) {
-            float g = 0.f;
-            if (kept) g = to_float(gy[r * gy_stride + col]);
-            if (gresidual) gresidual[r * outer + col] = from_float<T>(g);
-            if (kept) {
-                if (slope) g *= to_float(slope[r * outer + col]);
-                if (gz) {
-                    if constexpr (PLANES == 1) {
-                        reinterpret_cast<T *>(gz)[r * gz_stride + col] = from_float<T>(g);
-                    } else {
-                        bf16 piece[PLANES];
-                        split(g, piece);
+        constexpr int FLY = 4;
+        for (long long r0 = tile.begin + warp; r0 < tile.end; r0 += 8 * FLY) {
+            Pack<T, N> g[FLY];
+            Pack<Slope<T>, N> s[FLY];
 #pragma unroll
-                        for (int p = 0; p < PLANES; p++) reinterpret_cast<bf16 *>(gz)[(p * rows + r) * gz_stride + col] = piece[p];
-                    }
+            for (int u = 0; u < FLY; u++) {
+                const long long r = r0 + 8 * u;
+                if (kept && r < tile.end) {
+                    g[u] = *reinterpret_cast<const Pack<T, N> *>(gy + r * gy_stride + col);
+                    if (slope) s[u] = *reinterpret_cast<const Pack<Slope<T>, N> *>(slope + r * outer + col);
                 }
             }
-            sum += g;
+#pragma unroll
+            for (int u = 0; u < FLY; u++) {
+                const long long r = r0 + 8 * u;
+                if (r >= tile.end) break;
+                if (!kept) {
+                    if (gresidual) {
+#pragma unroll
+                        for (int n = 0; n < N; n++) g[u].v[n] = from_float<T>(0.f);
+                        *reinterpret_cast<Pack<T, N> *>(gresidual + r * outer + col) = g[u];
+                    }
+                    continue;
+                }
+                if (gresidual) *reinterpret_cast<Pack<T, N> *>(gresidual + r * outer + col) = g[u];
+                Pack<std::conditional_t<PLANES == 1, T, bf16>, N> pieces[PLANES];
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    float v = to_float(g[u].v[n]);
+                    if (slope) v *= to_float(s[u].v[n]);
+                    sum[n] += v;
+                    if constexpr (PLANES == 1) {
+                        pieces[0].v[n] = from_float<T>(v);
+                    } else {
+                        bf16 piece[PLANES];
+                        split(v, piece);
+#pragma unroll
+                        for (int p = 0; p < PLANES; p++) pieces[p].v[n] = piece[p];
+                    }
+                }
+                if (gz) {
+#pragma unroll
+                    for (int p = 0; p < PLANES; p++)
+                        *reinterpret_cast<decltype(&pieces[0])>(reinterpret_cast<decltype(&pieces[0].v[0])>(gz) + (p * rows + r) * gz_stride + col) = pieces[p];
+                }
+            }
         }
     }
     if (!part || !kept) return;
-    sums[warp][lane] = sum;
-    __syncthreads();
-    if (warp == 0 && col < outer) {
 #pragma unroll
-        for (int w = 1; w < 8; w++) sum += sums[w][lane];
-        part[(long long)blockIdx.x * outer + col] = sum;
+    for (int n = 0; n < N; n++) sums[warp][lane * N + n] = sum[n];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * N; i += blockDim.x) {
+        const int c = blockIdx.y * 32 * N + i;
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; w++) total += sums[w][i];
+        if (c < outer) part[(long long)blockIdx.x * outer + c] = total;
     }
 }
 
-// out[e][i] = sum of part[slab][i] over the slabs of group e, in ascending order
+// out[e][i] = sum of part[slab][i] over the slabs of group e, in ascending order: one or two such sums in a launch
 template <typename T>
-__global__ void __launch_bounds__(256) sum_slabs_kernel(T *__restrict__ out, const float *__restrict__ part, const int *__restrict__ offsets, long long rows, int height,
-                                                        long long size, long long slabs)
+struct SlabSum {
+    T *out;
+    const float *part;
+    long long size, slabs;        // of one group's result; slabs that part has room for
+    int height, blocks;           // blocks of the grid's x that belong to it
+};
+template <typename T, int N>
+__global__ void __launch_bounds__(256) sum_slabs_kernel(SlabSum<T> a, SlabSum<T> b, const int *__restrict__ offsets, long long rows)
 {
+    __shared__ long long first_slab;
     chain_wait();
     chain_release();
-    const int e = blockIdx.y;
-    const long long first = tiles_before(offsets, e, rows, height);
+    const bool second = (int)blockIdx.x >= a.blocks;
+    const SlabSum<T> &j = second ? b : a;
+    const int e = blockIdx.y, block = blockIdx.x - (second ? a.blocks : 0);
+    if (threadIdx.x < 32) {
+        const long long n = tiles_before(offsets, e, rows, j.height);
+        if (threadIdx.x == 0) first_slab = n;
+    }
+    __syncthreads();
     const RowRange r = group_rows(offsets, e, rows);
-    const long long n = min(tiles_of(r.end - r.begin, height), slabs - first);       // (`slabs` are there, whatever the offsets say)
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (long long)gridDim.x * blockDim.x) {
-        float sum = 0.f;
-        for (long long s = 0; s < n; s++) sum += part[(first + s) * size + i];
-        out[e * size + i] = from_float<T>(sum);
+    // (`slabs` are there, whatever the offsets say)
+    const int n = (int)min(tiles_of(r.end - r.begin, j.height), j.slabs - first_slab);
+    const float *part = j.part + first_slab * j.size;
+    for (long long i = ((long long)block * blockDim.x + threadIdx.x) * N; i < j.size; i += (long long)j.blocks * blockDim.x * N) {
+        float sum[N] = {};
+#pragma unroll 4
+        for (int s = 0; s < n; s++) {
+            const Pack<float, N> v = *reinterpret_cast<const Pack<float, N> *>(part + s * j.size + i);
+#pragma unroll
+            for (int c = 0; c < N; c++) sum[c] += v.v[c];
+        }
+        Pack<T, N> out;
+#pragma unroll
+        for (int c = 0; c < N; c++) out.v[c] = from_float<T>(sum[c]);
+        *reinterpret_cast<Pack<T, N> *>(j.out + e * j.size + i) = out;
     }
 }
 
@@ -439,11 +493,11 @@ struct WeightOut {
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 
-// Rows of a slab: enough slabs that the products of a slab keep all SMs busy, none shorter than 256 rows
-static int slab_height(long long rows, long long tiles_per_slab)
+// Rows of a slab: enough slabs that each SM gets `per_sm` of their tiles, none shorter than `least` rows
+static int slab_height(long long rows, long long tiles_per_slab, int per_sm, int least)
 {
-    long long slabs = (2LL * sm_count() + tiles_per_slab - 1) / tiles_per_slab;
-    if (slabs > (rows + 255) / 256) slabs = (rows + 255) / 256;
+    long long slabs = ((long long)per_sm * sm_count() + tiles_per_slab - 1) / tiles_per_slab;
+    if (slabs > (rows + least - 1) / least) slabs = (rows + least - 1) / least;
     if (slabs < 1) slabs = 1;
     const long long height = ((rows + slabs - 1) / slabs + 63) / 64 * 64;
     return (int)(height < 64 ? 64 : height > (1 << 30) ? (1 << 30) : height);
@@ -490,19 +544,27 @@ static ForwardPlan plan_forward(const ai2b_dense *d)
 
 struct BackwardPlan {
     bool tensor, slopes;
-    int weight_height, bias_height;
+    int weight_height, bias_height, vectors;
     PackedRows gz, x, weight;     // gz.copy: made by slope_kernel
     size_t weight_part, bias_part, total;
 };
 static int columns_of_tile(int dtype, int columns);
+
+// Columns that a lane of slope_kernel takes: 16 bytes of gy where all rows allow it (gz and the slopes are laid out to match), else one
+static int slope_vectors(const ai2b_dense *d)
+{
+    const long long size = (long long)element_bytes(d->dtype);
+    return common_alignment(d->d_gy, d->d_slope, d->d_gresidual, size * d->gy_stride, size * d->outer) >= 16 ? (int)(16 / size) : 1;
+}
 static BackwardPlan plan_backward(const ai2b_dense *d)
 {
     BackwardPlan p{};
     p.tensor = on_tensor_cores(d);
     p.slopes = d->activation != AI2B_ACT_NONE;
     const int bm = p.tensor ? tc::BM : FT, bn = p.tensor ? columns_of_tile(d->dtype, d->inner) : FT;
-    p.weight_height = slab_height(d->rows, (long long)((d->outer + bm - 1) / bm) * ((d->inner + bn - 1) / bn));
-    p.bias_height = slab_height(d->rows, (d->outer + 31) / 32);
+    p.weight_height = slab_height(d->rows, (long long)((d->outer + bm - 1) / bm) * ((d->inner + bn - 1) / bn), 2, 256);
+    p.vectors = slope_vectors(d);
+    p.bias_height = slab_height(d->rows, (d->outer + 32 * p.vectors - 1) / (32 * p.vectors), 8, 64);
     if (p.tensor) {
         p.gz = packed_rows(d->dtype, p.slopes ? nullptr : d->d_gy, p.slopes ? 1 : d->gy_stride, d->rows, d->outer, &p.total);
         p.x = packed_rows(d->dtype, d->d_x, d->x_stride, d->rows, d->inner, &p.total);
@@ -677,20 +739,16 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
         const bool products = d->rows > 0 && (d->d_gx || d->d_gweight), make_gz = products && p.gz.copy;
         float *wpart = (float *)(ws + p.weight_part), *bpart = (float *)(ws + p.bias_part);
         if (d->rows > 0 && (make_gz || d->d_gresidual || d->d_gbias)) {
-            const dim3 grid((unsigned)(slab_bound(d->rows, p.bias_height, d->groups) + 1), (d->outer + 31) / 32);
+            const dim3 grid((unsigned)(slab_bound(d->rows, p.bias_height, d->groups) + 1), (d->outer + 32 * p.vectors - 1) / (32 * p.vectors));
             auto go = [&](auto kern) {
                 return launch_chained(kern, grid, dim3(256), 0, st, make_gz ? (void *)(ws + p.gz.at) : (void *)nullptr, p.gz.stride(), (T *)d->d_gresidual,
                                       d->d_gbias ? bpart : (float *)nullptr, (const T *)d->d_gy, d->gy_stride,
                                       slopes ? (const Slope<T> *)d->d_slope : (const Slope<T> *)nullptr, d->d_offsets, d->groups, d->rows, p.bias_height, d->outer);
             };
+            constexpr int N = 16 / (int)sizeof(T);
             if constexpr (std::is_same<T, float>::value)
-                if (p.tensor) AI2B_CUDA(go(slope_kernel<float, 3>));
-            if (!(std::is_same<T, float>::value && p.tensor)) AI2B_CUDA(go(slope_kernel<T, 1>));
-        }
-        if (d->d_gbias) {
-            const dim3 grid((d->outer + 255) / 256, d->groups);
-            AI2B_CUDA(launch_chained(sum_slabs_kernel<T>, grid, dim3(256), 0, st, (T *)d->d_gbias, (const float *)bpart, d->d_offsets, d->rows, p.bias_height,
-                                     (long long)d->outer, slab_bound(d->rows, p.bias_height, d->groups)));
+                if (p.tensor) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<float, 3, N>) : go(slope_kernel<float, 3, 1>));
+            if (!(std::is_same<T, float>::value && p.tensor)) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<T, 1, N>) : go(slope_kernel<T, 1, 1>));
         }
         const T *gz = (const T *)(p.gz.copy ? ws + p.gz.at : d->d_gy);
         if (d->d_gx && d->rows > 0) {
@@ -715,10 +773,18 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
                 AI2B_CUDA(launch_chained(weight_fma_kernel<T>, grid, dim3(256), 0, st, gz, p.gz.stride(), (const T *)d->d_x, d->x_stride, d->d_offsets, d->groups, d->rows,
                                          p.weight_height, d->outer, d->inner, wpart));
             }
-            const long long size = (long long)d->outer * d->inner;
-            const dim3 grid((unsigned)((size + 255) / 256 < 4096 ? (size + 255) / 256 : 4096), d->groups);
-            AI2B_CUDA(launch_chained(sum_slabs_kernel<T>, grid, dim3(256), 0, st, (T *)d->d_gweight, (const float *)wpart, d->d_offsets, d->rows, p.weight_height, size,
-                                     slab_bound(d->rows, p.weight_height, d->groups)));
+        }
+        if (d->d_gweight || d->d_gbias) {
+            auto job = [&](void *to, const float *part, long long size, int height) {
+                const long long blocks = to ? (size + 1023) / 1024 : 0;
+                return SlabSum<T>{(T *)to, part, size, slab_bound(d->rows, height, d->groups), height, (int)(blocks < 2048 ? blocks : 2048)};
+            };
+            const SlabSum<T> w = job(d->d_gweight, wpart, (long long)d->outer * d->inner, p.weight_height), b = job(d->d_gbias, bpart, d->outer, p.bias_height);
+            const dim3 grid(w.blocks + b.blocks, d->groups);
+            const bool fours = (d->d_gweight ? d->outer * (long long)d->inner % 4 == 0 : true) && d->outer % 4 == 0 &&
+                               common_alignment(d->d_gweight, d->d_gbias) >= 4 * (int)sizeof(T);
+            if (fours) AI2B_CUDA(launch_chained(sum_slabs_kernel<T, 4>, grid, dim3(256), 0, st, w, b, d->d_offsets, d->rows));
+            else AI2B_CUDA(launch_chained(sum_slabs_kernel<T, 1>, grid, dim3(256), 0, st, w, b, d->d_offsets, d->rows));
         }
         return (int)AI2B_OK;
     });

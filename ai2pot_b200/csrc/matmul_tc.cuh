@@ -9,8 +9,13 @@
 // operand is transposed.
 //
 // More digits than 16 bits hold come in planes: a matrix as a sum of PLANES 16-bit matrices, hi + mid (+ lo), each a further piece of the
-// significand. The product is the sum of the plane products of order below PLANES (1, 3 or 6 of them), added up in the same float accumulator;
-// a stage holds all planes of its tiles, so each is loaded once.
+// significand. The product is the sum of the plane products of order below PLANES (1, 3 or 6 of them); a stage holds all planes of its
+// tiles, so each is loaded once.
+//
+// The accumulator is a float that is cut, not rounded, after every 16 of the summed index: 2^-24 of the sum is lost each time, always towards
+// zero (6.6e-6 after 96 such steps, 1.1e-3 at 65536 x 6 products, measured on sums of positive numbers). That is below the rounding of a 16-bit result.
+// With planes the digits count: the products of lower order go into an accumulator of their own, where what is cut is 2^-8 (2^-11) times as
+// large, and both are taken out and added up in registers, with rounding, after every two stages.
 //
 // Every wait ends: after WAIT_LIMIT tries a role gives up, the block waits (bounded again) for its copies and products in flight, frees its
 // TMEM, raises a flag that ai2b_fitnet_check() reports, and returns.
@@ -26,7 +31,7 @@ constexpr int EPILOGUE_WARPS = 8, THREADS = 64 + 32 * EPILOGUE_WARPS;
 constexpr int STAGE_LIMIT = 8;
 constexpr int STAGING_BYTES = EPILOGUE_WARPS * 32 * 32 * 4;      // per epilogue warp 32 rows x 32 columns of float
 constexpr int SMEM_BUDGET = 227 * 1024;
-constexpr int WAIT_LIMIT = 1 << 22;
+constexpr int WAIT_LIMIT = 1 << 20;
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------------
 
@@ -110,6 +115,10 @@ struct Shape {
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
     static constexpr int STAGES_FIT = (SMEM_BUDGET - STAGING_BYTES - 2048) / STAGE_BYTES;
     static constexpr int STAGES = STAGES_FIT < STAGE_LIMIT ? STAGES_FIT : STAGE_LIMIT;
+    static constexpr bool CAREFUL = PLANES > 1;
+    static constexpr int ACCUMULATORS = CAREFUL ? 2 : 1, CHUNK = CAREFUL ? 2 * BK : 1 << 30;      // of the summed index per accumulation
+    static constexpr int TMEM_COLUMNS = 2 * ACCUMULATORS * BN;
+    static_assert(TMEM_COLUMNS <= 512, "two sets of accumulators in TMEM");
     static constexpr int SMEM = STAGES * STAGE_BYTES + STAGING_BYTES + 2048;      // with 1024 bytes to align by and 1024 for barriers
     static_assert(STAGES >= 2, "two stages at least");
 };
@@ -146,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     unsigned *tmem_slot = reinterpret_cast<unsigned *>(smem + (drained + 8 - base));
     int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int TMEM_COLUMNS = 2 * BN;
+    constexpr int TMEM_COLUMNS = S::TMEM_COLUMNS;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) {
@@ -197,92 +206,124 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     } else if (warp == 1) {
         const unsigned idesc = instruction_descriptor(ops.is_bf16, A_MN, B_MN, BN);
         Item it;
-        unsigned used = 0, tile = 0;
+        unsigned used = 0, sets = 0;          // sets of accumulators begun
         for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
-            if (it.k_begin >= it.k_end) continue;
-            const unsigned buf = tile & 1, d = tmem + buf * BN;
-            if (tile >= 2) ok = barrier_wait(taken + 8 * buf, ((tile >> 1) - 1) & 1);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int k = it.k_begin; k < it.k_end; k += BK, used++) {
-                const unsigned s = used % S::STAGES;
-                ok = barrier_wait(full + 8 * s, (used / S::STAGES) & 1);
+            for (int k0 = it.k_begin; ok && k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end) {
+                const unsigned set = sets & 1, d = tmem + set * S::ACCUMULATORS * BN;
+                if (sets >= 2) ok = barrier_wait(taken + 8 * set, ((sets >> 1) - 1) & 1);
                 if (!ok) break;
-                const unsigned a = base + s * S::STAGE_BYTES, b = a + PLANES * S::A_BYTES;
-                const int left = it.k_end - k, steps = left >= BK ? BK / 16 : (left + 15) / 16;
-                if constexpr (A_MN && B_MN) {
-                    // The summed index runs over rows of memory, and what follows k_end may belong to another network: it may hold NaN, so it
-                    // is zeroed in both operands up to the 16 rows of the last step. A row is 128 whole bytes whatever the swizzle.
-                    if (left < steps * 16) {
-                        for (int i = lane; i < (steps * 16 - left) * 8; i += 32) {
-                            const unsigned at = (left + (i >> 3)) * 128 + (i & 7) * 16;
-                            for (int c = 0; c < PLANES * (BM + BN) / 64; c++)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a + c * BK * 128 + at), "r"(0) : "memory");
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                    }
-                }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (lane == 0) {
-                    for (int step = 0; step < steps; step++) {
-                        // 16 of the summed index: 32 bytes along a K-major row, 16 rows of an MN-major tile
-                        const unsigned a_step = step * (A_MN ? 16 * 128 : 32), b_step = step * (B_MN ? 16 * 128 : 32);
-                        bool more = k > it.k_begin || step > 0;
+                for (int k = k0; k < it.k_end && (!S::CAREFUL || k < k0 + S::CHUNK); k += BK, used++) {
+                    const unsigned s = used % S::STAGES;
+                    ok = barrier_wait(full + 8 * s, (used / S::STAGES) & 1);
+                    if (!ok) break;
+                    const unsigned a = base + s * S::STAGE_BYTES, b = a + PLANES * S::A_BYTES;
+                    const int left = it.k_end - k, steps = left >= BK ? BK / 16 : (left + 15) / 16;
+                    if constexpr (A_MN && B_MN) {
+                        // The summed index runs over rows of memory, and what follows k_end may belong to another network: it may hold NaN, so
+                        // it is zeroed in both operands up to the 16 rows of the last step. A row is 128 whole bytes whatever the swizzle.
+                        if (left < steps * 16) {
+                            for (int i = lane; i < (steps * 16 - left) * 8; i += 32) {
+                                const unsigned at = (left + (i >> 3)) * 128 + (i & 7) * 16;
+                                for (int c = 0; c < PLANES * (BM + BN) / 64; c++)
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a + c * BK * 128 + at), "r"(0) : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                        }
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (lane == 0) {
+                        for (int step = 0; step < steps; step++) {
+                            // 16 of the summed index: 32 bytes along a K-major row, 16 rows of an MN-major tile
+                            const unsigned a_step = step * (A_MN ? 16 * 128 : 32), b_step = step * (B_MN ? 16 * 128 : 32);
+                            const bool more = k > k0 || step > 0;
 #pragma unroll
-                        for (int order = PLANES - 1; order >= 0; order--) {      // small pieces first
+                            for (int order = PLANES - 1; order >= 0; order--) {      // small pieces first
 #pragma unroll
-                            for (int pa = 0; pa <= order; pa++) {
-                                mma(d, tile_descriptor(a + pa * S::A_BYTES + a_step, BK * 128), tile_descriptor(b + (order - pa) * S::B_BYTES + b_step, BK * 128), idesc, more);
-                                more = true;
+                                for (int pa = 0; pa <= order; pa++)
+                                    mma(order > 0 ? d + BN : d, tile_descriptor(a + pa * S::A_BYTES + a_step, BK * 128),
+                                        tile_descriptor(b + (order - pa) * S::B_BYTES + b_step, BK * 128), idesc, order == 0 ? more : more || order < PLANES - 1 || pa > 0);
                             }
                         }
+                        commit(empty + 8 * s);
                     }
-                    commit(empty + 8 * s);
+                    __syncwarp();
                 }
+                if (!ok) break;
+                if (lane == 0) commit(done + 8 * set);
                 __syncwarp();
+                sets++;
             }
-            if (!ok) break;
-            if (lane == 0) commit(done + 8 * buf);
-            __syncwarp();
-            tile++;
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         float *mine = staging + (warp - 2) * 1024;
         Item it;
-        unsigned tile = 0;
+        unsigned sets = 0;
+        // Lane l holds row l of 32 sums: through shared memory, so that neighbouring lanes get neighbouring columns. Four columns at a time, permuted
+        // within the row, keep both directions free of bank conflicts.
+        auto hand_over = [&](const float (&v)[32], long long row, int col) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                *reinterpret_cast<float4 *>(mine + 32 * lane + 4 * (i ^ (lane & 7))) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            __syncwarp();
+            out(it, row, col, mine, lane);
+            __syncwarp();
+        };
         for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
-            const bool sums = it.k_begin < it.k_end;
-            const unsigned buf = tile & 1;
-            if (sums) {
-                ok = barrier_wait(done + 8 * buf, (tile >> 1) & 1);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            }
             const long long row = it.row + 32 * quarter;
-            for (int c = 32 * half; c < BN; c += 64) {
-                if (row >= it.row_end || it.col + c >= out.columns) break;
-                float v[32];
-                if (sums) {
-                    tmem_load32(v, tmem + buf * BN + c + ((unsigned)(32 * quarter) << 16));
-                } else {
+            float sum[S::CAREFUL ? BN / 64 : 1][32];
+            if constexpr (S::CAREFUL) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = 0.f;
+                for (int i = 0; i < BN / 64; i++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++) sum[i][j] = 0.f;
+                for (int k0 = it.k_begin; k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end, sets++) {
+                    ok = barrier_wait(done + 8 * (sets & 1), (sets >> 1) & 1);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned from = tmem + (sets & 1) * S::ACCUMULATORS * BN + 32 * half + ((unsigned)(32 * quarter) << 16);
+#pragma unroll
+                    for (int i = 0; i < BN / 64; i++) {
+                        float v[32], low[32];
+                        tmem_load32(v, from + 64 * i);
+                        tmem_load32(low, from + BN + 64 * i);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) sum[i][j] += v[j] + low[j];
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    if (lane == 0) barrier_arrive(taken + 8 * (sets & 1));
                 }
-                // Lane l holds row l: through shared memory, so that neighbouring lanes get neighbouring columns. Four columns at a time,
-                // permuted within the row, keep both directions free of bank conflicts.
+                if (!ok) break;
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    *reinterpret_cast<float4 *>(mine + 32 * lane + 4 * (i ^ (lane & 7))) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                __syncwarp();
-                out(it, row, it.col + c, mine, lane);
-                __syncwarp();
-            }
-            if (sums) {
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                if (lane == 0) barrier_arrive(taken + 8 * buf);
-                tile++;
+                for (int i = 0; i < BN / 64; i++) {
+                    const int c = 32 * half + 64 * i;
+                    if (row < it.row_end && it.col + c < out.columns) hand_over(sum[i], row, it.col + c);
+                }
+            } else {
+                const bool sums = it.k_begin < it.k_end;
+                const unsigned set = sets & 1;
+                if (sums) {
+                    ok = barrier_wait(done + 8 * set, (sets >> 1) & 1);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
+                for (int c = 32 * half; c < BN; c += 64) {
+                    if (row >= it.row_end || it.col + c >= out.columns) break;
+                    if (sums) {
+                        tmem_load32(sum[0], tmem + set * BN + c + ((unsigned)(32 * quarter) << 16));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) sum[0][j] = 0.f;
+                    }
+                    hand_over(sum[0], row, it.col + c);
+                }
+                if (sums) {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    if (lane == 0) barrier_arrive(taken + 8 * set);
+                    sets++;
+                }
             }
         }
     }
