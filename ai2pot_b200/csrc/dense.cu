@@ -33,8 +33,16 @@ __device__ __forceinline__ Activated activate(float z)
         const float p = QUICK ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
         return {z * p, p * (1.f + z * (1.f - p))};
     } else if constexpr (ACT == AI2B_ACT_GELU) {
-        const float p = QUICK ? fmaf(0.5f, erff(0.70710678118654752f * z), 0.5f) : 0.5f * erfcf(-0.70710678118654752f * z);
-        return {z * p, fmaf(z * 0.39894228040143268f, QUICK ? __expf(-0.5f * z * z) : expf(-0.5f * z * z), p)};
+        if constexpr (QUICK) {
+            // Phi(-|z|) = e^(-z^2/2) (a1 t + ... + a5 t^5) / 2, t = 1 / (1 + p |z| / sqrt 2): Abramowitz and Stegun 7.1.26, off by 7.5e-8 at most; the
+            // exponential is the slope's as well. (27 us less on 65536 x 1024 than erff.)
+            const float e = __expf(-0.5f * z * z), t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+            const float tail = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+            const float p = z > 0.f ? 1.f - tail : tail;
+            return {z * p, fmaf(z * 0.39894228040143268f, e, p)};
+        }
+        const float p = 0.5f * erfcf(-0.70710678118654752f * z);
+        return {z * p, fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), p)};
     } else {
         return {z, 1.f};
     }
@@ -339,22 +347,93 @@ __global__ void __launch_bounds__(256) sum_slabs_kernel(SlabSum<T> a, SlabSum<T>
 // ---- products on the tensor cores -------------------------------------------------------------------------------------------
 
 // Tiles of 128 rows x BN columns of one group each; the columns of a row tile follow each other, so that its rows are read from memory once
+// The groups' tiles of `height` rows, found through two tables in shared memory: the first tile of each group, then its first row (made to ascend
+// whatever the offsets hold)
+struct GroupTable {
+    const int *offsets;
+    int groups, height;
+    long long rows;
+    __device__ __forceinline__ void prepare(int *table) const
+    {
+        if (!offsets) return;
+        if (threadIdx.x < 32) {
+            int *first = table, *row = table + groups + 1;
+            int base = 0, end = 0;
+            for (int e0 = 0; e0 < groups; e0 += 32) {
+                const int e = e0 + (int)threadIdx.x;
+                int to = e < groups ? (int)group_rows(offsets, e, rows).end : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(FULL_MASK, to, o);
+                    if ((int)threadIdx.x >= o) to = max(to, up);
+                }
+                to = max(to, end);
+                int from = __shfl_up_sync(FULL_MASK, to, 1);
+                if (threadIdx.x == 0) from = end;
+                const int mine = (int)tiles_of(to - from, height);
+                int scan = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(FULL_MASK, scan, o);
+                    if ((int)threadIdx.x >= o) scan += up;
+                }
+                if (e < groups) {
+                    first[e] = base + scan - mine;
+                    row[e] = from;
+                }
+                base += __shfl_sync(FULL_MASK, scan, 31);
+                end = __shfl_sync(FULL_MASK, to, 31);
+            }
+            if (threadIdx.x == 0) {
+                first[groups] = base;
+                row[groups] = end;
+            }
+        }
+        __syncthreads();
+    }
+    // whole warps; as find_tile
+    __device__ __forceinline__ RowTile find(const int *table, long long tile) const
+    {
+        if (!offsets) {
+            const long long row = tile * height;
+            return row < rows ? RowTile{0, row, min(row + height, rows)} : RowTile{-1, 0, 0};
+        }
+        if (!table) return find_tile(offsets, groups, rows, height, tile);
+        const int *first = table, *row = table + groups + 1;
+        if (tile >= first[groups]) {
+            const long long at = row[groups] + (tile - first[groups]) * height;
+            return at < rows ? RowTile{groups, at, min(at + height, rows)} : RowTile{-1, 0, 0};
+        }
+        // the last group whose first tile is not behind `tile` (groups without rows share theirs with the next one)
+        int e = 0;
+        for (int e0 = 0; e0 < groups; e0 += 32) {
+            const int i = e0 + (int)(threadIdx.x & 31);
+            const unsigned before = __ballot_sync(FULL_MASK, i < groups && first[i] <= tile);
+            if (!before) break;
+            e = e0 + 31 - __clz(before);
+        }
+        const long long at = row[e] + (tile - first[e]) * height;
+        return RowTile{e, at, min(at + height, (long long)row[e + 1])};
+    }
+};
+
+// Tiles of 128 rows x BN columns of one group each; the columns of a row tile follow each other, so that its rows are read from memory once
 template <int BN>
 struct RowItems {
-    const int *offsets;
-    int groups, column_tiles, inner;
-    long long rows;
-    __device__ __forceinline__ bool get(long long t, tc::Item &it) const
+    GroupTable of;
+    int column_tiles, inner;
+    __device__ __forceinline__ void prepare(int *table) const { of.prepare(table); }
+    __device__ __forceinline__ bool get(const int *table, long long t, tc::Item &it) const
     {
-        const long long m = t / column_tiles;
-        const RowTile tile = find_tile(offsets, groups, rows, tc::BM, m);
+        const long long m = row_of(t, column_tiles, t <= 0xffffffffLL);
+        const RowTile tile = of.find(table, m);
         if (tile.group < 0) return false;
         it.a_at = (int)tile.begin;
         it.a_batch = 0;
         it.b_at = it.col = (int)(t - m * column_tiles) * BN;
         it.b_batch = tile.group;
         it.k_begin = 0;
-        it.k_end = tile.group < groups ? inner : 0;
+        it.k_end = tile.group < of.groups ? inner : 0;
         it.row = tile.begin;
         it.row_end = tile.end;
         it.batch = tile.group;
@@ -367,11 +446,34 @@ template <typename T>
 struct RowOut {
     RowOutput<T> o;
     int columns, groups;
-    bool vectors;             // all rows start at multiples of 16 bytes and end at whole vectors
+    bool vectors, bias_vectors;      // all rows (and those of the bias) start at multiples of 16 bytes and end at whole vectors
 
     static constexpr int N = 16 / (int)sizeof(T), LANES = 32 / N, ROWS = 32 / LANES;      // a lane takes N columns of every ROWS-th row
+
+    struct Ahead {
+        Pack<T, N> residual, bias;      // of the first pass
+    };
+    __device__ __forceinline__ Pack<T, N> read(const T *p, int col, bool whole) const
+    {
+        Pack<T, N> v;
+        if (whole) {
+            v = *reinterpret_cast<const Pack<T, N> *>(p);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) v.v[j] = col + j < columns ? p[j] : from_float<T>(0.f);
+        }
+        return v;
+    }
+    __device__ __forceinline__ void load(Ahead &a, const tc::Item &it, long long row, int col0, int lane) const
+    {
+        const int col = col0 + lane % LANES * N;
+        if (it.batch >= groups || col >= columns) return;
+        if (o.bias) a.bias = read(o.bias + (long long)it.batch * columns + col, col, vectors && bias_vectors);
+        if (o.residual) a.residual = read(o.residual + min(row + lane / LANES, it.row_end - 1) * o.residual_stride + col, col, vectors);
+    }
+
     template <int ACT>
-    __device__ __forceinline__ void apply(const tc::Item &it, long long row, int col0, const float *mine, int lane) const
+    __device__ __forceinline__ void apply(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &ahead) const
     {
         constexpr bool QUICK = sizeof(T) == 2;
         const int i0 = lane % LANES * N, col = col0 + i0, n = min(N, columns - col);
@@ -380,26 +482,19 @@ struct RowOut {
         float bias[N] = {};
         if (o.bias && kept) {
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if (j < n) bias[j] = to_float(o.bias[(long long)it.batch * columns + col + j]);
+            for (int j = 0; j < N; j++) bias[j] = to_float(ahead.bias.v[j]);
         }
-#pragma unroll 4
-        for (int r = lane / LANES; r < 32; r += ROWS) {
-            const long long at = row + r;
-            if (at >= it.row_end) return;
-            float z[N], residual[N] = {};
-            if (o.residual && kept) {
-                const T *p = o.residual + at * o.residual_stride + col;
-                if (vectors) {
-                    const Pack<T, N> v = *reinterpret_cast<const Pack<T, N> *>(p);
-#pragma unroll
-                    for (int j = 0; j < N; j++) residual[j] = to_float(v.v[j]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < N; j++)
-                        if (j < n) residual[j] = to_float(p[j]);
-                }
-            }
+        const int last = (int)min((long long)32, it.row_end - row);
+        T *py = o.out + (row + lane / LANES) * columns + col;
+        Slope<T> *ps = o.slope + (row + lane / LANES) * columns + col;
+        const bool add = o.residual && kept;
+        Pack<T, N> residual, next = ahead.residual;
+        // not unrolled: a small call runs this code once, and has to fetch all of it (1157 x 131 x 97: 20 us unrolled)
+#pragma unroll 1
+        for (int r = lane / LANES; r < last; r += ROWS, py += ROWS * (long long)columns, ps += ROWS * (long long)columns) {
+            residual = next;
+            if (add && r + ROWS < last) next = read(o.residual + (row + r + ROWS) * o.residual_stride + col, col, vectors);
+            float z[N];
 #pragma unroll
             for (int j = 0; j < N; j += 4) {
                 const float4 s = tc::staged(mine, r, (i0 + j) / 4);
@@ -412,32 +507,30 @@ struct RowOut {
             Pack<Slope<T>, N> slope;
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                const Activated a = kept ? activate<ACT, QUICK>(z[j]) : Activated{0.f, 0.f};
-                y.v[j] = from_float<T>(a.value + residual[j]);
+                const Activated a = activate<ACT, QUICK>(z[j]);      // (0 for 0, whichever it is)
+                y.v[j] = from_float<T>(add ? a.value + to_float(residual.v[j]) : a.value);
                 slope.v[j] = from_float<Slope<T>>(a.slope);
             }
-            T *py = o.out + at * columns + col;
-            Slope<T> *ps = o.slope ? o.slope + at * columns + col : nullptr;
             if (vectors) {
                 *reinterpret_cast<Pack<T, N> *>(py) = y;
-                if (ps) *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
+                if (o.slope) *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
             } else {
 #pragma unroll
                 for (int j = 0; j < N; j++)
                     if (j < n) {
                         py[j] = y.v[j];
-                        if (ps) ps[j] = slope.v[j];
+                        if (o.slope) ps[j] = slope.v[j];
                     }
             }
         }
     }
-    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col, const float *mine, int lane) const
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col, const float *mine, int lane, const Ahead &ahead) const
     {
         switch (o.activation) {
-        case AI2B_ACT_TANH: apply<AI2B_ACT_TANH>(it, row, col, mine, lane); break;
-        case AI2B_ACT_SILU: apply<AI2B_ACT_SILU>(it, row, col, mine, lane); break;
-        case AI2B_ACT_GELU: apply<AI2B_ACT_GELU>(it, row, col, mine, lane); break;
-        default: apply<AI2B_ACT_NONE>(it, row, col, mine, lane);
+        case AI2B_ACT_TANH: apply<AI2B_ACT_TANH>(it, row, col, mine, lane, ahead); break;
+        case AI2B_ACT_SILU: apply<AI2B_ACT_SILU>(it, row, col, mine, lane, ahead); break;
+        case AI2B_ACT_GELU: apply<AI2B_ACT_GELU>(it, row, col, mine, lane, ahead); break;
+        default: apply<AI2B_ACT_NONE>(it, row, col, mine, lane, ahead);
         }
     }
 };
@@ -445,15 +538,15 @@ struct RowOut {
 // Tiles of gz^T x over the rows of one slab
 template <int BN>
 struct WeightItems {
-    const int *offsets;
-    int groups, height, row_tiles, column_tiles, outer;
-    long long rows;
-    __device__ __forceinline__ bool get(long long t, tc::Item &it) const
+    GroupTable of;
+    int row_tiles, column_tiles, outer;
+    __device__ __forceinline__ void prepare(int *table) const { of.prepare(table); }
+    __device__ __forceinline__ bool get(const int *table, long long t, tc::Item &it) const
     {
         const int per_slab = row_tiles * column_tiles;
-        const long long slab = t / per_slab;
-        const RowTile tile = find_tile(offsets, groups, rows, height, slab);
-        if (tile.group < 0 || tile.group >= groups) return false;
+        const long long slab = row_of(t, per_slab, t <= 0xffffffffLL);
+        const RowTile tile = of.find(table, slab);
+        if (tile.group < 0 || tile.group >= of.groups) return false;
         const int i = (int)(t - slab * per_slab);
         it.a_at = i / column_tiles * tc::BM;
         it.b_at = it.col = i % column_tiles * BN;
@@ -470,7 +563,9 @@ struct WeightOut {
     float *part;              // [slab][outer][inner]
     int columns, outer;
     bool vectors;
-    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane) const
+    struct Ahead {};
+    __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &) const
     {
         const int i = lane & 7, col = col0 + 4 * i;
         if (col >= columns) return;
@@ -641,8 +736,8 @@ static int multiply_rows(const ai2b_dense *d, const PackedRows &a, const PackedR
         ops.a_stack = 1;
         ops.b_stack = d->groups;
         ops.is_bf16 = d->dtype != AI2B_F16;
-        const RowItems<BN> items{d->d_offsets, d->groups, (columns + BN - 1) / BN, inner, d->rows};
-        const RowOut<T> out{o, columns, d->groups, rows_in_vectors(o, columns)};
+        const RowItems<BN> items{{d->d_offsets, d->groups, tc::BM, d->rows}, (columns + BN - 1) / BN, inner};
+        const RowOut<T> out{o, columns, d->groups, rows_in_vectors(o, columns), common_alignment(o.bias) >= 16};
         return tc::launch<PLANES, BN, false, B_MN>(ops, items, out, ((d->rows + tc::BM - 1) / tc::BM + d->groups) * items.column_tiles, st);
     });
 }
@@ -660,7 +755,7 @@ static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const uns
         if (rc != AI2B_OK) return rc;
         ops.a_stack = ops.b_stack = 1;
         ops.is_bf16 = d->dtype != AI2B_F16;
-        const WeightItems<BN> items{d->d_offsets, d->groups, p.weight_height, (d->outer + tc::BM - 1) / tc::BM, (d->inner + BN - 1) / BN, d->outer, d->rows};
+        const WeightItems<BN> items{{d->d_offsets, d->groups, p.weight_height, d->rows}, (d->outer + tc::BM - 1) / tc::BM, (d->inner + BN - 1) / BN, d->outer};
         const WeightOut out{part, d->inner, d->outer, d->inner % 4 == 0};
         return tc::launch<PLANES, BN, true, true>(ops, items, out, slab_bound(d->rows, p.weight_height, d->groups) * items.row_tiles * items.column_tiles, st);
     });

@@ -45,6 +45,10 @@ inline int common_alignment(N... n)
     return (int)(all & (~all + 1));
 }
 
+// i / d; a division of 64-bit numbers takes several times as long as the rest of a thread's arithmetic, so it is made of 32 bits where
+// the whole range fits
+__device__ __forceinline__ long long row_of(long long i, int d, bool narrow) { return narrow ? (long long)((unsigned)i / (unsigned)d) : i / d; }
+
 // Offsets come from device memory that the host has not seen: whatever they hold, the rows of group e are [begin, end) inside [0, rows].
 struct RowRange {
     long long begin, end;

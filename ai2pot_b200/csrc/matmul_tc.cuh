@@ -1,7 +1,7 @@
 // Matrix products on the fifth-generation tensor cores, for the fitting-network kernels.
 //
 // One persistent block per SM. A producer warp copies operand tiles to shared memory with TMA, one thread of a second warp issues
-// tcgen05.mma into one of two accumulators in TMEM, eight warps take finished accumulators out and hand them to an epilogue while
+// tcgen05.mma into one of two accumulators in TMEM, the other warps take finished accumulators out and hand them to an epilogue while
 // the next tile is being multiplied. Tiles are 128 x BN, 64 of the summed index per stage.
 //
 // Operands are 16-bit matrices in memory with 16-byte aligned rows, read in the direction that they lie in: an operand whose rows run
@@ -27,10 +27,9 @@ namespace ai2b {
 namespace tc {
 
 constexpr int BM = 128, BK = 64;
-constexpr int EPILOGUE_WARPS = 8, THREADS = 64 + 32 * EPILOGUE_WARPS;
 constexpr int STAGE_LIMIT = 8;
-constexpr int STAGING_BYTES = EPILOGUE_WARPS * 32 * 32 * 4;      // per epilogue warp 32 rows x 32 columns of float
 constexpr int SMEM_BUDGET = 227 * 1024;
+constexpr int TABLE_BYTES = 8 * 1032;         // what Items may keep in shared memory
 constexpr int WAIT_LIMIT = 1 << 20;
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------------
@@ -113,13 +112,20 @@ template <int PLANES, int BN>
 struct Shape {
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;      // one plane
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
-    static constexpr int STAGES_FIT = (SMEM_BUDGET - STAGING_BYTES - 2048) / STAGE_BYTES;
-    static constexpr int STAGES = STAGES_FIT < STAGE_LIMIT ? STAGES_FIT : STAGE_LIMIT;
     static constexpr bool CAREFUL = PLANES > 1;
+    // Sixteen epilogue warps: an activation with its slope is a chain of some 40 dependent instructions, and two warps per scheduler left it
+    // idle four cycles of five (13824 x 512 x 512 with silu: 40 us with eight warps). With planes the products take several times as long, and the
+    // stages need the memory that eight more warps would stage their sums in.
+    static constexpr int EPILOGUE_WARPS = CAREFUL ? 8 : 16, SHARES = EPILOGUE_WARPS / 4, THREADS = 64 + 32 * EPILOGUE_WARPS;
+    static constexpr int STAGING_BYTES = EPILOGUE_WARPS * 32 * 32 * 4;      // per epilogue warp 32 rows x 32 columns of float
+    static constexpr bool TABLE = !CAREFUL;      // (two stages of three planes leave no room)
+    static constexpr int OTHER_BYTES = (TABLE ? TABLE_BYTES : 0) + 2048;          // with 1024 bytes to align by and 1024 for barriers
+    static constexpr int STAGES_FIT = (SMEM_BUDGET - STAGING_BYTES - OTHER_BYTES) / STAGE_BYTES;
+    static constexpr int STAGES = STAGES_FIT < STAGE_LIMIT ? STAGES_FIT : STAGE_LIMIT;
     static constexpr int ACCUMULATORS = CAREFUL ? 2 : 1, CHUNK = CAREFUL ? 2 * BK : 1 << 30;      // of the summed index per accumulation
     static constexpr int TMEM_COLUMNS = 2 * ACCUMULATORS * BN;
     static_assert(TMEM_COLUMNS <= 512, "two sets of accumulators in TMEM");
-    static constexpr int SMEM = STAGES * STAGE_BYTES + STAGING_BYTES + 2048;      // with 1024 bytes to align by and 1024 for barriers
+    static constexpr int SMEM = STAGES * STAGE_BYTES + STAGING_BYTES + OTHER_BYTES;
     static_assert(STAGES >= 2, "two stages at least");
 };
 
@@ -141,19 +147,22 @@ struct Operands {
     int *gave_up;                 // set by a wait that ran out
 };
 
-// Tiles: Items::get(long long t, Item &) by whole warps, false after the last one. Out: out(item, lane quarter's row, column, accumulators).
+// Items::prepare(table), by all threads, may leave something in shared memory; Items::get(table, t, item), by whole warps, gives tile t, false after
+// the last one. (table is NULL, and nothing was prepared, where there is no room for it.) Out takes 32 x 32 sums at a time, in shared memory:
+// out.load(ahead, item, first row, first column, lane) reads what it needs of memory, out(item, first row, first column, sums, lane, ahead) stores.
 template <int PLANES, int BN, bool A_MN, bool B_MN, typename Items, typename Out>
-__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Operands ops, const __grid_constant__ Items items, const __grid_constant__ Out out)
+__global__ void __launch_bounds__(Shape<PLANES, BN>::THREADS, 1) product_kernel(const __grid_constant__ Operands ops, const __grid_constant__ Items items, const __grid_constant__ Out out)
 {
     using S = Shape<PLANES, BN>;
     extern __shared__ unsigned char smem_raw[];
     const unsigned raw = smem_address(smem_raw), base = (raw + 1023) & ~1023u;
     unsigned char *smem = smem_raw + (base - raw);
     float *staging = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE_BYTES);
-    const unsigned bars = base + S::STAGES * S::STAGE_BYTES + STAGING_BYTES;
+    const unsigned bars = base + S::STAGES * S::STAGE_BYTES + S::STAGING_BYTES;
     const unsigned full = bars, empty = bars + 8 * STAGE_LIMIT, done = empty + 8 * STAGE_LIMIT, taken = done + 16, drained = taken + 16;
     unsigned *tmem_slot = reinterpret_cast<unsigned *>(smem + (drained + 8 - base));
     int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
+    int *table = S::TABLE ? reinterpret_cast<int *>(smem + (bars + 1024 - base)) : nullptr;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int TMEM_COLUMNS = S::TMEM_COLUMNS;
 
@@ -164,7 +173,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         }
         for (int b = 0; b < 2; b++) {
             barrier_init(done + 8 * b, 1);
-            barrier_init(taken + 8 * b, EPILOGUE_WARPS);
+            barrier_init(taken + 8 * b, S::EPILOGUE_WARPS);
         }
         barrier_init(drained, 1);
         *stopped = 0;
@@ -181,12 +190,13 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     const unsigned tmem = *tmem_slot;
     chain_wait();
     chain_release();
+    if (S::TABLE) items.prepare(table);
 
     bool ok = true;
     unsigned issued = 0;                 // stages that the producer has started
     if (warp == 0) {
         Item it;
-        for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
+        for (long long t = blockIdx.x; ok && items.get(table, t, it); t += gridDim.x) {
             for (int k = it.k_begin; ok && k < it.k_end; k += BK, issued++) {
                 const unsigned s = issued % S::STAGES, round = issued / S::STAGES;
                 ok = round == 0 || barrier_wait(empty + 8 * s, (round - 1) & 1);
@@ -207,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         const unsigned idesc = instruction_descriptor(ops.is_bf16, A_MN, B_MN, BN);
         Item it;
         unsigned used = 0, sets = 0;          // sets of accumulators begun
-        for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
+        for (long long t = blockIdx.x; ok && items.get(table, t, it); t += gridDim.x) {
             for (int k0 = it.k_begin; ok && k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end) {
                 const unsigned set = sets & 1, d = tmem + set * S::ACCUMULATORS * BN;
                 if (sets >= 2) ok = barrier_wait(taken + 8 * set, ((sets >> 1) - 1) & 1);
@@ -257,38 +267,40 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             }
         }
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int quarter = warp & 3, share = (warp - 2) >> 2;      // rows 32 * quarter.., columns 32 * share.. of every 32 * SHARES
         float *mine = staging + (warp - 2) * 1024;
         Item it;
         unsigned sets = 0;
         // Lane l holds row l of 32 sums: through shared memory, so that neighbouring lanes get neighbouring columns. Four columns at a time, permuted
         // within the row, keep both directions free of bank conflicts.
-        auto hand_over = [&](const float (&v)[32], long long row, int col) {
+        auto hand_over = [&](const float (&v)[32], long long row, int col, const typename Out::Ahead &ahead) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 *reinterpret_cast<float4 *>(mine + 32 * lane + 4 * (i ^ (lane & 7))) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             __syncwarp();
-            out(it, row, col, mine, lane);
+            out(it, row, col, mine, lane, ahead);
             __syncwarp();
         };
-        for (long long t = blockIdx.x; ok && items.get(t, it); t += gridDim.x) {
+        for (long long t = blockIdx.x; ok && items.get(table, t, it); t += gridDim.x) {
             const long long row = it.row + 32 * quarter;
-            float sum[S::CAREFUL ? BN / 64 : 1][32];
+            constexpr int PARTS = (BN + 32 * S::SHARES - 1) / (32 * S::SHARES);
+            float sum[S::CAREFUL ? PARTS : 1][32];
             if constexpr (S::CAREFUL) {
 #pragma unroll
-                for (int i = 0; i < BN / 64; i++)
+                for (int i = 0; i < PARTS; i++)
 #pragma unroll
                     for (int j = 0; j < 32; j++) sum[i][j] = 0.f;
                 for (int k0 = it.k_begin; k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end, sets++) {
                     ok = barrier_wait(done + 8 * (sets & 1), (sets >> 1) & 1);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned from = tmem + (sets & 1) * S::ACCUMULATORS * BN + 32 * half + ((unsigned)(32 * quarter) << 16);
+                    const unsigned from = tmem + (sets & 1) * S::ACCUMULATORS * BN + 32 * share + ((unsigned)(32 * quarter) << 16);
 #pragma unroll
-                    for (int i = 0; i < BN / 64; i++) {
+                    for (int i = 0; i < PARTS; i++) {
+                        if (32 * (share + S::SHARES * i) >= BN) break;
                         float v[32], low[32];
-                        tmem_load32(v, from + 64 * i);
-                        tmem_load32(low, from + BN + 64 * i);
+                        tmem_load32(v, from + 32 * S::SHARES * i);
+                        tmem_load32(low, from + BN + 32 * S::SHARES * i);
 #pragma unroll
                         for (int j = 0; j < 32; j++) sum[i][j] += v[j] + low[j];
                     }
@@ -297,27 +309,36 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int i = 0; i < BN / 64; i++) {
-                    const int c = 32 * half + 64 * i;
-                    if (row < it.row_end && it.col + c < out.columns) hand_over(sum[i], row, it.col + c);
+                for (int i = 0; i < PARTS; i++) {
+                    const int c = 32 * (share + S::SHARES * i);
+                    if (c < BN && row < it.row_end && it.col + c < out.columns) {
+                        typename Out::Ahead ahead;
+                        out.load(ahead, it, row, it.col + c, lane);
+                        hand_over(sum[i], row, it.col + c, ahead);
+                    }
                 }
             } else {
                 const bool sums = it.k_begin < it.k_end;
                 const unsigned set = sets & 1;
+                // What the epilogue reads of memory is asked for before the sums are there. (For the columns after the first 32 there are no registers
+                // to do it while those are worked on.)
+                typename Out::Ahead ahead;
+                if (32 * share < BN && row < it.row_end && it.col + 32 * share < out.columns) out.load(ahead, it, row, it.col + 32 * share, lane);
                 if (sums) {
                     ok = barrier_wait(done + 8 * set, (sets >> 1) & 1);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
-                for (int c = 32 * half; c < BN; c += 64) {
+                for (int c = 32 * share; c < BN; c += 32 * S::SHARES) {
                     if (row >= it.row_end || it.col + c >= out.columns) break;
+                    if (c != 32 * share) out.load(ahead, it, row, it.col + c, lane);
                     if (sums) {
                         tmem_load32(sum[0], tmem + set * BN + c + ((unsigned)(32 * quarter) << 16));
                     } else {
 #pragma unroll
                         for (int j = 0; j < 32; j++) sum[0][j] = 0.f;
                     }
-                    hand_over(sum[0], row, it.col + c);
+                    hand_over(sum[0], row, it.col + c, ahead);
                 }
                 if (sums) {
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -367,7 +388,7 @@ int launch(const Operands &ops, const Items &items, const Out &out, long long ti
     const int rc = kernel_setup(ks, kern, S::SMEM);
     if (rc != AI2B_OK) return rc;
     const int sms = sm_count();
-    AI2B_CUDA(launch_chained(kern, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(THREADS), S::SMEM, st, ops, items, out));
+    AI2B_CUDA(launch_chained(kern, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(S::THREADS), S::SMEM, st, ops, items, out));
     return AI2B_OK;
 }
 

@@ -139,10 +139,6 @@ route_place_kernel(const I *__restrict__ index, long long nslots, long long run,
     }
 }
 
-// i / d; a division of 64-bit numbers takes several times as long as the rest of a thread's arithmetic, so it is made of 32 bits where
-// the whole range fits
-__device__ __forceinline__ long long row_of(long long i, int d, bool narrow) { return narrow ? (long long)((unsigned)i / (unsigned)d) : i / d; }
-
 // Thread i of the grid moves access i % per_row of row i / per_row, then the same UNROLL - 1 more times a grid further on: that many
 // loads are in flight at once.
 template <typename V, int UNROLL>
