@@ -21,32 +21,100 @@ constexpr int MAX_GROUPS = 1024;
 struct Activated {
     float value, slope;
 };
-// QUICK: for results that are rounded to 16 bits. Exponentials and quotients of hardware precision (a few 2^-23), and the error of Phi is
-// absolute, not relative, in its lower tail: below 2^-20 of 1 + |z| in either case.
-template <int ACT, bool QUICK>
+template <int ACT>
 __device__ __forceinline__ Activated activate(float z)
 {
     if constexpr (ACT == AI2B_ACT_TANH) {
-        const float t = QUICK ? 1.f - __fdividef(2.f, 1.f + __expf(2.f * z)) : tanhf(z);      // (an exponential that overflows gives a quotient of zero)
+        const float t = tanhf(z);
         return {t, 1.f - t * t};
     } else if constexpr (ACT == AI2B_ACT_SILU) {
-        const float p = QUICK ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
+        const float p = 1.f / (1.f + expf(-z));
         return {z * p, p * (1.f + z * (1.f - p))};
     } else if constexpr (ACT == AI2B_ACT_GELU) {
-        if constexpr (QUICK) {
-            // Phi(-|z|) = e^(-z^2/2) (a1 t + ... + a5 t^5) / 2, t = 1 / (1 + p |z| / sqrt 2): Abramowitz and Stegun 7.1.26, off by 7.5e-8 at most; the
-            // exponential is the slope's as well. (27 us less on 65536 x 1024 than erff.)
-            const float e = __expf(-0.5f * z * z), t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
-            const float tail = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-            const float p = z > 0.f ? 1.f - tail : tail;
-            return {z * p, fmaf(z * 0.39894228040143268f, e, p)};
-        }
         const float p = 0.5f * erfcf(-0.70710678118654752f * z);
         return {z * p, fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), p)};
     } else {
         return {z, 1.f};
     }
 }
+
+// The same for results that are rounded to 16 bits, two at a time: the epilogue of a 16-bit layer is bound by the instructions that it issues
+// (39 per element with one at a time and expf's handling of subnormal numbers: 10,000 cycles for a tile whose products take 4,000).
+// Errors stay below 2^-20 of 1 + |z|.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)), "l"(reinterpret_cast<const unsigned long long &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 exp2_2(float2 a)
+{
+    float2 d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.x) : "f"(a.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.y) : "f"(a.y));
+    return d;
+}
+__device__ __forceinline__ float2 rcp2(float2 a)
+{
+    float2 d;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d.x) : "f"(a.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d.y) : "f"(a.y));
+    return d;
+}
+struct Activated2 {
+    float2 value, slope;
+};
+constexpr float LOG2_E = 1.4426950408889634f;
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ Activated2 activate2(float2 z)
+{
+    Activated2 a{z, both(1.f)};
+    if constexpr (ACT == AI2B_ACT_TANH) {
+        const float2 r = rcp2(add2(exp2_2(mul2(z, both(2.f * LOG2_E))), both(1.f)));      // (an exponential that overflows gives a reciprocal of zero)
+        a.value = fma2(r, both(-2.f), both(1.f));
+        if constexpr (SLOPE) a.slope = fma2(mul2(a.value, both(-1.f)), a.value, both(1.f));
+    } else if constexpr (ACT == AI2B_ACT_SILU) {
+        const float2 p = rcp2(add2(exp2_2(mul2(z, both(-LOG2_E))), both(1.f)));
+        a.value = mul2(z, p);
+        if constexpr (SLOPE) a.slope = fma2(a.value, fma2(p, both(-1.f), both(1.f)), p);
+    } else if constexpr (ACT == AI2B_ACT_GELU) {
+        // Phi(-|z|) = e^(-z^2/2) (a1 t + ... + a5 t^5) / 2, t = 1 / (1 + p |z| / sqrt 2): Abramowitz and Stegun 7.1.26, off by 7.5e-8 at most; the
+        // exponential is the slope's as well
+        const float2 size = make_float2(fabsf(z.x), fabsf(z.y)), e = exp2_2(mul2(mul2(z, z), both(-0.5f * LOG2_E)));
+        const float2 t = rcp2(fma2(size, both(0.3275911f * 0.70710678118654752f), both(1.f)));
+        float2 q = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+        q = fma2(t, q, both(0.5f * 1.421413741f));
+        q = fma2(t, q, both(0.5f * -0.284496736f));
+        q = fma2(t, q, both(0.5f * 0.254829592f));
+        const float2 tail = mul2(mul2(q, t), e);
+        a.value = fma2(mul2(size, both(-1.f)), tail, make_float2(z.x > 0.f ? z.x : 0.f * z.x, z.y > 0.f ? z.y : 0.f * z.y));
+        if constexpr (SLOPE) {
+            const float2 above = fma2(tail, both(-1.f), both(1.f));
+            a.slope = fma2(mul2(z, both(0.39894228040143268f)), e, make_float2(z.x > 0.f ? above.x : tail.x, z.y > 0.f ? above.y : tail.y));
+        }
+    }
+    return a;
+}
+
+__device__ __forceinline__ float2 widen(bf16 a, bf16 b) { return make_float2(__bfloat162float(a), __bfloat162float(b)); }
+__device__ __forceinline__ float2 widen(f16 a, f16 b) { return __half22float2(__halves2half2(a, b)); }
+__device__ __forceinline__ void narrow(bf16 *to, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(to) = __float22bfloat162_rn(v); }
+__device__ __forceinline__ void narrow(f16 *to, float2 v) { *reinterpret_cast<__half2 *>(to) = __float22half2_rn(v); }
 
 // ---- tiles of rows --------------------------------------------------------------------------------------------------------
 
@@ -125,10 +193,10 @@ __device__ __forceinline__ void store_row_element(const RowOutput<T> &o, long lo
     if (o.bias) z += to_float(o.bias[(long long)group * columns + col]);
     Activated a;
     switch (o.activation) {
-    case AI2B_ACT_TANH: a = activate<AI2B_ACT_TANH, false>(z); break;
-    case AI2B_ACT_SILU: a = activate<AI2B_ACT_SILU, false>(z); break;
-    case AI2B_ACT_GELU: a = activate<AI2B_ACT_GELU, false>(z); break;
-    default: a = activate<AI2B_ACT_NONE, false>(z);
+    case AI2B_ACT_TANH: a = activate<AI2B_ACT_TANH>(z); break;
+    case AI2B_ACT_SILU: a = activate<AI2B_ACT_SILU>(z); break;
+    case AI2B_ACT_GELU: a = activate<AI2B_ACT_GELU>(z); break;
+    default: a = activate<AI2B_ACT_NONE>(z);
     }
     if (o.slope) o.slope[row * columns + col] = from_float<Slope<T>>(a.slope);
     if (o.residual) a.value += to_float(o.residual[row * o.residual_stride + col]);
@@ -472,65 +540,79 @@ struct RowOut {
         if (o.residual) a.residual = read(o.residual + min(row + lane / LANES, it.row_end - 1) * o.residual_stride + col, col, vectors);
     }
 
-    template <int ACT>
+    template <int ACT, bool SLOPE>
     __device__ __forceinline__ void apply(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &ahead) const
     {
-        constexpr bool QUICK = sizeof(T) == 2;
         const int i0 = lane % LANES * N, col = col0 + i0, n = min(N, columns - col);
         if (n <= 0) return;
-        const bool kept = it.batch < groups;
-        float bias[N] = {};
-        if (o.bias && kept) {
+        const bool kept = it.batch < groups, add = o.residual && kept;
+        float2 bias[N / 2];
 #pragma unroll
-            for (int j = 0; j < N; j++) bias[j] = to_float(ahead.bias.v[j]);
+        for (int j = 0; j < N / 2; j++) {
+            if constexpr (sizeof(T) == 4) bias[j] = make_float2(ahead.bias.v[2 * j], ahead.bias.v[2 * j + 1]);
+            else bias[j] = widen(ahead.bias.v[2 * j], ahead.bias.v[2 * j + 1]);
+            if (!o.bias || !kept) bias[j] = both(0.f);
         }
         const int last = (int)min((long long)32, it.row_end - row);
         T *py = o.out + (row + lane / LANES) * columns + col;
-        Slope<T> *ps = o.slope + (row + lane / LANES) * columns + col;
-        const bool add = o.residual && kept;
+        Slope<T> *ps = SLOPE ? o.slope + (row + lane / LANES) * columns + col : nullptr;
         Pack<T, N> residual, next = ahead.residual;
-        // not unrolled: a small call runs this code once, and has to fetch all of it (1157 x 131 x 97: 20 us unrolled)
+        // not unrolled: a small call runs this code once, and has to fetch all of it
 #pragma unroll 1
-        for (int r = lane / LANES; r < last; r += ROWS, py += ROWS * (long long)columns, ps += ROWS * (long long)columns) {
+        for (int r = lane / LANES; r < last; r += ROWS, py += ROWS * (long long)columns) {
             residual = next;
             if (add && r + ROWS < last) next = read(o.residual + (row + r + ROWS) * o.residual_stride + col, col, vectors);
-            float z[N];
+            float2 z[N / 2];
 #pragma unroll
             for (int j = 0; j < N; j += 4) {
                 const float4 s = tc::staged(mine, r, (i0 + j) / 4);
-                z[j] = s.x + bias[j];
-                z[j + 1] = s.y + bias[j + 1];
-                z[j + 2] = s.z + bias[j + 2];
-                z[j + 3] = s.w + bias[j + 3];
+                z[j / 2] = add2(make_float2(s.x, s.y), bias[j / 2]);
+                z[j / 2 + 1] = add2(make_float2(s.z, s.w), bias[j / 2 + 1]);
             }
             Pack<T, N> y;
             Pack<Slope<T>, N> slope;
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const Activated a = activate<ACT, QUICK>(z[j]);      // (0 for 0, whichever it is)
-                y.v[j] = from_float<T>(add ? a.value + to_float(residual.v[j]) : a.value);
-                slope.v[j] = from_float<Slope<T>>(a.slope);
+            for (int j = 0; j < N; j += 2) {
+                if constexpr (sizeof(T) == 4) {
+                    const Activated a = activate<ACT>(z[j / 2].x), b = activate<ACT>(z[j / 2].y);
+                    y.v[j] = add ? a.value + residual.v[j] : a.value;
+                    y.v[j + 1] = add ? b.value + residual.v[j + 1] : b.value;
+                    slope.v[j] = a.slope;
+                    slope.v[j + 1] = b.slope;
+                } else {
+                    Activated2 a = activate2<ACT, SLOPE>(z[j / 2]);
+                    if (add) a.value = add2(a.value, widen(residual.v[j], residual.v[j + 1]));
+                    narrow(&y.v[j], a.value);
+                    if constexpr (SLOPE) narrow(&slope.v[j], a.slope);
+                }
             }
             if (vectors) {
                 *reinterpret_cast<Pack<T, N> *>(py) = y;
-                if (o.slope) *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
+                if constexpr (SLOPE) *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
             } else {
 #pragma unroll
                 for (int j = 0; j < N; j++)
                     if (j < n) {
                         py[j] = y.v[j];
-                        if (o.slope) ps[j] = slope.v[j];
+                        if constexpr (SLOPE) ps[j] = slope.v[j];
                     }
             }
+            if constexpr (SLOPE) ps += ROWS * (long long)columns;
         }
+    }
+    template <int ACT>
+    __device__ __forceinline__ void choose(const tc::Item &it, long long row, int col, const float *mine, int lane, const Ahead &ahead) const
+    {
+        if (ACT != AI2B_ACT_NONE && o.slope) apply<ACT, true>(it, row, col, mine, lane, ahead);
+        else apply<ACT, false>(it, row, col, mine, lane, ahead);
     }
     __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col, const float *mine, int lane, const Ahead &ahead) const
     {
         switch (o.activation) {
-        case AI2B_ACT_TANH: apply<AI2B_ACT_TANH>(it, row, col, mine, lane, ahead); break;
-        case AI2B_ACT_SILU: apply<AI2B_ACT_SILU>(it, row, col, mine, lane, ahead); break;
-        case AI2B_ACT_GELU: apply<AI2B_ACT_GELU>(it, row, col, mine, lane, ahead); break;
-        default: apply<AI2B_ACT_NONE>(it, row, col, mine, lane, ahead);
+        case AI2B_ACT_TANH: choose<AI2B_ACT_TANH>(it, row, col, mine, lane, ahead); break;
+        case AI2B_ACT_SILU: choose<AI2B_ACT_SILU>(it, row, col, mine, lane, ahead); break;
+        case AI2B_ACT_GELU: choose<AI2B_ACT_GELU>(it, row, col, mine, lane, ahead); break;
+        default: choose<AI2B_ACT_NONE>(it, row, col, mine, lane, ahead);
         }
     }
 };
