@@ -2,10 +2,17 @@
 //
 //   X = G / (|G|_F + eps);  steps times:  A = X X^T,  X = a X + (b A + c A A) X      (m <= n; else A = X^T X and X = a X + X (b A + c A A))
 //
-// The iteration acts on each singular value alone, sigma -> a sigma + b sigma^3 + c sigma^5, so X is carried in float: what a rounding
-// of X adds to directions of small singular values is multiplied by up to a^steps.
+// The iteration acts on each singular value alone, sigma -> a sigma + b sigma^3 + c sigma^5. What a rounding of X adds to directions of
+// small singular values is multiplied by up to a^steps, so X is carried in 22 digits and more: in float, or as two halves. The products
+// (b A + c A A) X are another matter: their rounding errors come multiplied by A or X, so that they turn a singular direction by their own relative
+// size but do not grow. bfloat16 updates (8 digits) therefore multiply single halves (11 digits; error against 64 bits 0.0020 of the result's
+// norm, 0.0017 of it the result's rounding), float and half ones the two halves of each factor (22 digits): with single ones a half result is off
+// by 0.0012 to 0.0027, five times its rounding.
+//
+// A and b A + c A A are symmetric: only tiles on and above the diagonal are multiplied, and stored twice.
 #include "fitnet.cuh"
 #include "fma_tile.cuh"
+#include "matmul_tc.cuh"
 
 namespace ai2b {
 
@@ -71,24 +78,165 @@ __global__ void __launch_bounds__(256) product_fma_kernel(T *__restrict__ out, f
         }
 }
 
+// ---- on the tensor cores ----------------------------------------------------------------------------------------------------
+
+// A number v is kept as halves of SCALE v: hi, and lo = what hi leaves. X has singular values of about one at most, so that its elements are
+// near 1 / sqrt(rows) in size; SCALE keeps lo a normal number there, and numbers up to 1000 in range.
+constexpr float SCALE = 64.f;
+__device__ __forceinline__ void halves(float v, f16 &hi, f16 &lo)
+{
+    v *= SCALE;
+    hi = __float2half_rn(v);
+    lo = __float2half_rn(v - __half2float(hi));
+}
+
+// X0 = G / (|G| + eps) as halves, rows padded to `stride`
+template <typename T>
+__global__ void __launch_bounds__(256) normalise_halves_kernel(f16 *__restrict__ hi, f16 *__restrict__ lo, long long stride, const T *__restrict__ g, int m, int n, int parts,
+                                                               const double *__restrict__ part, double eps)
+{
+    chain_wait();
+    chain_release();
+    double sum = 0.0;
+    for (int i = 0; i < parts; i++) sum += part[blockIdx.y * NORM_BLOCKS + i];
+    const double scale = 1.0 / (sqrt(sum) + eps);
+    const long long size = (long long)m * n;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (long long)gridDim.x * blockDim.x) {
+        const long long r = row_of(i, n, size <= 0xffffffffLL), at = (blockIdx.y * (long long)m + r) * stride + (i - r * n);
+        halves((float)((double)to_float(g[blockIdx.y * size + i]) * scale), hi[at], lo[at]);
+    }
+}
+
+// 128 x BN tiles of a batch of products; with `symmetric` (BN = 128) those on and above the diagonal
+template <int BN>
+struct BatchItems {
+    int row_tiles, column_tiles, inner, rows, batch;
+    bool symmetric;
+    __device__ __forceinline__ void prepare(int *) const {}
+    __device__ __forceinline__ bool get(const int *, long long t, tc::Item &it) const
+    {
+        const int per = symmetric ? row_tiles * (row_tiles + 1) / 2 : row_tiles * column_tiles;
+        const int b = (int)(t / per);
+        if (b >= batch) return false;
+        int i = (int)(t - (long long)b * per), r = 0;
+        if (symmetric) {
+            // rows of the triangle hold row_tiles, row_tiles - 1, ... tiles
+            const float n = row_tiles + 0.5f;
+            r = max(0, (int)(n - sqrtf(fmaxf(n * n - 2.f * i, 0.f))) - 1);
+            while (i >= (r + 1) * row_tiles - (r + 1) * r / 2) r++;
+            i = i - (r * row_tiles - r * (r - 1) / 2) + r;
+        } else {
+            r = i / column_tiles;
+            i -= r * column_tiles;
+        }
+        it.a_at = r * tc::BM;
+        it.b_at = it.col = i * BN;
+        it.a_batch = it.b_batch = it.batch = b;
+        it.k_begin = 0;
+        it.k_end = inner;
+        it.row = it.a_at;
+        it.row_end = rows;
+        return true;
+    }
+};
+
+// v = beta sums + alpha d; stored as halves, or, at the last step, as the result. d: halves of a matrix laid out like the result.
+template <typename T, bool FINAL>
+struct BatchOut {
+    float alpha, beta;                    // (of the scaled numbers)
+    const f16 *d_hi, *d_lo;               // NULL: nothing to add; d_lo NULL: one half only
+    f16 *hi, *lo;                         // lo NULL: not kept
+    T *result;
+    int columns, rows;
+    long long stride;                     // of the halves' rows, a multiple of 8
+    bool symmetric;
+
+    struct Ahead {};
+    __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &) const
+    {
+        const int i0 = lane % 4 * 8, col = col0 + i0;
+        const long long matrix = (long long)it.batch * rows;
+        if (col < columns) {
+#pragma unroll 1
+            for (int r = lane / 4; r < 32 && row + r < it.row_end; r += 8) {
+                const float4 s0 = tc::staged(mine, r, i0 / 4), s1 = tc::staged(mine, r, i0 / 4 + 1);
+                const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+                store(s, matrix + row + r, col, columns);
+            }
+        }
+        if (symmetric && it.a_at != it.b_at) {
+            // rows and columns exchanged: eight rows of the sums make up a piece of a row
+            const int r0 = lane % 4 * 8;
+#pragma unroll 1
+            for (int c = lane / 4; c < 32 && col0 + c < columns; c += 8) {
+                if (row + r0 >= it.row_end) break;
+                float s[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) s[j] = mine[32 * (r0 + j) + 4 * ((c / 4) ^ ((r0 + j) & 7)) + c % 4];
+                store(s, matrix + col0 + c, (int)row + r0, columns);
+            }
+        }
+    }
+    // columns [col, col + 8) of one row of the result; rows of the halves are padded to whole eights
+    __device__ __forceinline__ void store(const float (&s)[8], long long row, int col, int end) const
+    {
+        float v[8];
+        Pack<f16, 8> p, q;
+        const long long at = row * stride + col;
+        if (d_hi) {
+            p = *reinterpret_cast<const Pack<f16, 8> *>(d_hi + at);
+            if (d_lo) q = *reinterpret_cast<const Pack<f16, 8> *>(d_lo + at);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            v[j] = beta * s[j];
+            if (d_hi) v[j] = fmaf(alpha, __half2float(p.v[j]) + (d_lo ? __half2float(q.v[j]) : 0.f), v[j]);
+        }
+        if constexpr (FINAL) {
+            T *to = result + row * columns + col;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (col + j < end) to[j] = from_float<T>(v[j] * (1.f / SCALE));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                p.v[j] = __float2half_rn(v[j]);
+                q.v[j] = __float2half_rn(v[j] - __half2float(p.v[j]));
+            }
+            *reinterpret_cast<Pack<f16, 8> *>(hi + at) = p;
+            if (lo) *reinterpret_cast<Pack<f16, 8> *>(lo + at) = q;
+        }
+    }
+};
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+
+// The FMA pipes take matrices that a single tile would hold most of
+static bool on_tensor_cores(int m, int n) { return (double)m * n * (m < n ? m : n) >= 5e5; }
+static long long padded(long long n) { return (n + 7) / 8 * 8; }
+
 struct OrthogonalizePlan {
     size_t norm, x[2], gram, poly, total;
 };
 static OrthogonalizePlan plan_orthogonalize(int batch, int m, int n)
 {
     OrthogonalizePlan p{};
-    const size_t s = m < n ? m : n;
+    const long long s = m < n ? m : n;
+    const bool tensor = on_tensor_cores(m, n);
+    // (two halves are as large as a float)
+    const size_t xs = sizeof(float) * (size_t)batch * m * (tensor ? padded(n) : n), ss = sizeof(float) * (size_t)batch * s * (tensor ? padded(s) : s);
     size_t at = 0;
     p.norm = at;
     at += round256(sizeof(double) * (size_t)batch * NORM_BLOCKS);
     for (int i = 0; i < 2; i++) {
         p.x[i] = at;
-        at += round256(sizeof(float) * (size_t)batch * m * n);
+        at += round256(xs);
     }
     p.gram = at;
-    at += round256(sizeof(float) * (size_t)batch * s * s);
+    at += round256(ss);
     p.poly = at;
-    at += round256(sizeof(float) * (size_t)batch * s * s);
+    at += round256(ss);
     p.total = at;
     return p;
 }
@@ -101,6 +249,61 @@ static int product(T *out, float alpha, const float *d, float beta, Operand<floa
     return AI2B_OK;
 }
 
+// Halves of a batch of matrices: hi of all of them, then lo of all of them
+struct Halves {
+    f16 *hi, *lo;
+    int rows, columns;
+    long long stride;
+};
+
+// result[b] (rows x columns) = beta A[b] B[b]^T + alpha d[b]. A_MN, B_MN: the operand lies transposed.
+template <int PLANES, bool A_MN, bool B_MN, typename Out>
+static int product_tc(const Halves &a, const Halves &b, const Out &out, int inner, int batch, cudaStream_t st)
+{
+    // float: two planes of 128 columns fill the accumulators. Symmetric products want square tiles.
+    auto go = [&](auto bn) {
+        constexpr int BN = decltype(bn)::value;
+        tc::Operands ops{};
+        int rc = tc::make_map(&ops.a, a.hi, false, a.columns, a.rows, (long long)batch * PLANES, a.stride, a.rows * a.stride, A_MN ? 64 : tc::BM);
+        if (rc == AI2B_OK) rc = tc::make_map(&ops.b, b.hi, false, b.columns, b.rows, (long long)batch * PLANES, b.stride, b.rows * b.stride, B_MN ? 64 : BN);
+        if (rc == AI2B_OK) rc = tc::flag_address(&ops.gave_up);
+        if (rc != AI2B_OK) return rc;
+        ops.a_stack = ops.b_stack = batch;
+        const BatchItems<BN> items{(out.rows + tc::BM - 1) / tc::BM, (out.columns + BN - 1) / BN, inner, out.rows, batch, out.symmetric};
+        const long long per = out.symmetric ? (long long)items.row_tiles * (items.row_tiles + 1) / 2 : (long long)items.row_tiles * items.column_tiles;
+        return tc::launch<PLANES, BN, A_MN, B_MN>(ops, items, out, per * batch, st);
+    };
+    if constexpr (PLANES == 1)
+        if (!out.symmetric && (long long)batch * ((out.rows + 127) / 128) * ((out.columns + 255) / 256) >= sm_count()) return go(std::integral_constant<int, 256>{});
+    return go(std::integral_constant<int, 128>{});
+}
+
+// The iteration on halves: PLANES of them are multiplied
+template <typename T, int PLANES, bool WIDE>
+static int iterate_tc(T *result, Halves x, Halves next, const Halves &gram, const Halves &poly, int steps, float a, float b, float c, int batch, cudaStream_t st)
+{
+    const int m = x.rows, n = x.columns, s = gram.rows, l = WIDE ? n : m;
+    constexpr bool TWO = PLANES == 2;
+    constexpr float UNSCALE = 1.f / SCALE;      // a product of two scaled numbers has one scale too many
+    for (int i = 0; i < steps; i++) {
+        const BatchOut<T, false> to_gram{0.f, UNSCALE, nullptr, nullptr, gram.hi, TWO ? gram.lo : nullptr, nullptr, s, s, gram.stride, true};
+        const BatchOut<T, false> to_poly{b, c * UNSCALE, gram.hi, TWO ? gram.lo : nullptr, poly.hi, TWO ? poly.lo : nullptr, nullptr, s, s, poly.stride, true};
+        const BatchOut<T, false> to_next{a, UNSCALE, x.hi, x.lo, next.hi, next.lo, nullptr, n, m, x.stride, false};
+        const BatchOut<T, true> to_result{a, UNSCALE, x.hi, x.lo, nullptr, nullptr, result, n, m, x.stride, false};
+        int rc = product_tc<PLANES, !WIDE, !WIDE>(x, x, to_gram, l, batch, st);
+        if (rc == AI2B_OK) rc = product_tc<PLANES, false, false>(gram, gram, to_poly, s, batch, st);
+        if (rc == AI2B_OK) {
+            // m <= n: poly X, with X's rows along the summed index; else X poly, where poly is its own transpose
+            const Halves &left = WIDE ? poly : x, &right = WIDE ? x : poly;
+            if (i + 1 < steps) rc = product_tc<PLANES, false, WIDE>(left, right, to_next, s, batch, st);
+            else rc = product_tc<PLANES, false, WIDE>(left, right, to_result, s, batch, st);
+        }
+        if (rc != AI2B_OK) return rc;
+        std::swap(x, next);
+    }
+    return AI2B_OK;
+}
+
 }  // namespace ai2b
 
 using namespace ai2b;
@@ -108,7 +311,7 @@ using namespace ai2b;
 extern "C" size_t ai2b_orthogonalize_workspace_bytes(int dtype, int batch, int m, int n)
 {
     if (!known_dtype(dtype) || batch < 1 || m < 1 || n < 1) return 256;
-    return plan_orthogonalize(batch, m, n).total + 256;
+    return plan_orthogonalize(batch, m, n).total;
 }
 
 extern "C" int ai2b_orthogonalize(int dtype, void *d_out, const void *d_g, int batch, int m, int n, int steps, double a, double b, double c, double eps, void *d_workspace,
@@ -129,9 +332,22 @@ extern "C" int ai2b_orthogonalize(int dtype, void *d_out, const void *d_g, int b
         const long long size = (long long)m * n;
         const int s = m < n ? m : n, parts = (int)(size < NORM_BLOCKS * 1024LL ? (size + 1023) / 1024 : NORM_BLOCKS);
         double *norm = (double *)(ws + p.norm);
+        const bool tensor = on_tensor_cores(m, n) && steps > 0;
         float *x = (float *)(ws + p.x[0]), *next = (float *)(ws + p.x[1]), *gram = (float *)(ws + p.gram), *poly = (float *)(ws + p.poly);
         AI2B_CUDA(launch_chained(norm_kernel<T>, dim3(parts, batch), dim3(256), 0, st, (const T *)d_g, size, norm));
         const int blocks = (int)(size < 512 * 256LL ? (size + 255) / 256 : 512);
+        if (tensor) {
+            auto halves_of = [&](float *at, int rows, int columns) {
+                const long long stride = padded(columns);
+                return Halves{(f16 *)at, (f16 *)at + batch * rows * stride, rows, columns, stride};
+            };
+            const Halves x0 = halves_of(x, m, n), x1 = halves_of(next, m, n), g = halves_of(gram, s, s), q = halves_of(poly, s, s);
+            AI2B_CUDA(launch_chained(normalise_halves_kernel<T>, dim3(blocks, batch), dim3(256), 0, st, x0.hi, x0.lo, x0.stride, (const T *)d_g, m, n, parts, (const double *)norm,
+                                     eps));
+            constexpr int PLANES = std::is_same<T, bf16>::value ? 1 : 2;
+            return m <= n ? iterate_tc<T, PLANES, true>((T *)d_out, x0, x1, g, q, steps, (float)a, (float)b, (float)c, batch, st)
+                          : iterate_tc<T, PLANES, false>((T *)d_out, x0, x1, g, q, steps, (float)a, (float)b, (float)c, batch, st);
+        }
         AI2B_CUDA(launch_chained(normalise_kernel<T>, dim3(blocks, batch), dim3(256), 0, st, x, (const T *)d_g, size, parts, (const double *)norm, eps));
         const long long ss = (long long)s * s;
         for (int i = 0; i < steps; i++) {
