@@ -621,7 +621,7 @@ struct RowOut {
 template <int BN>
 struct WeightItems {
     GroupTable of;
-    int row_tiles, column_tiles, outer;
+    int tile_rows, row_tiles, column_tiles, outer;
     __device__ __forceinline__ void prepare(int *table) const { of.prepare(table); }
     __device__ __forceinline__ bool get(const int *table, long long t, tc::Item &it) const
     {
@@ -630,7 +630,7 @@ struct WeightItems {
         const RowTile tile = of.find(table, slab);
         if (tile.group < 0 || tile.group >= of.groups) return false;
         const int i = (int)(t - slab * per_slab);
-        it.a_at = i / column_tiles * tc::BM;
+        it.a_at = i / column_tiles * tile_rows;
         it.b_at = it.col = i % column_tiles * BN;
         it.a_batch = it.b_batch = 0;
         it.k_begin = (int)tile.begin;
@@ -722,10 +722,10 @@ static ForwardPlan plan_forward(const ai2b_dense *d)
 struct BackwardPlan {
     bool tensor, slopes;
     int weight_height, bias_height, vectors;
+    tc::Tile weight_tile;
     PackedRows gz, x, weight;     // gz.copy: made by slope_kernel
     size_t weight_part, bias_part, total;
 };
-static int columns_of_tile(int dtype, int columns);
 
 // Columns that a lane of slope_kernel takes: 16 bytes of gy where all rows allow it (gz and the slopes are laid out to match), else one
 static int slope_vectors(const ai2b_dense *d)
@@ -738,8 +738,14 @@ static BackwardPlan plan_backward(const ai2b_dense *d)
     BackwardPlan p{};
     p.tensor = on_tensor_cores(d);
     p.slopes = d->activation != AI2B_ACT_NONE;
-    const int bm = p.tensor ? tc::BM : FT, bn = p.tensor ? columns_of_tile(d->dtype, d->inner) : FT;
-    p.weight_height = slab_height(d->rows, (long long)((d->outer + bm - 1) / bm) * ((d->inner + bn - 1) / bn), 2, 256);
+    if (p.tensor) {
+        // tiles of a slab of 2048 rows, as many slabs as there are
+        p.weight_tile = tc::best_tile(planes_of(d->dtype), d->outer, 0, d->inner, (d->rows + 2047) / 2048, 2048, sm_count());
+        const int bm = p.weight_tile.rows(), bn = p.weight_tile.columns;
+        p.weight_height = slab_height(d->rows, (long long)((d->outer + bm - 1) / bm) * ((d->inner + bn - 1) / bn) * (p.weight_tile.pair ? 2 : 1), 2, 256);
+    } else {
+        p.weight_height = slab_height(d->rows, (long long)((d->outer + FT - 1) / FT) * ((d->inner + FT - 1) / FT), 2, 256);
+    }
     p.vectors = slope_vectors(d);
     p.bias_height = slab_height(d->rows, (d->outer + 32 * p.vectors - 1) / (32 * p.vectors), 8, 64);
     if (p.tensor) {
@@ -777,26 +783,6 @@ static int map_rows(CUtensorMap *map, int dtype, const PackedRows &p, const unsi
     return tc::make_map(map, p.copy ? ws + p.at : p.from, dtype != AI2B_F16, p.columns, rows, batch * planes_of(dtype), p.stride(), rows * p.stride(), box_rows);
 }
 
-// Columns of a tile: the width that wastes the fewest columns, and the wider of two that waste as many. Three planes of 256 columns do not
-// fit two stages.
-static int columns_of_tile(int dtype, int columns)
-{
-    int best = 64;
-    for (int bn = 128; bn <= (dtype == AI2B_F32 ? 128 : 256); bn *= 2)
-        if ((columns + bn - 1) / bn * bn <= (columns + best - 1) / best * best) best = bn;
-    return best;
-}
-
-// f(integral_constant<BN>)
-template <typename T, typename F>
-static int with_columns(int bn, F &&f)
-{
-    if (bn == 64) return f(std::integral_constant<int, 64>{});
-    if constexpr (sizeof(T) == 2)
-        if (bn == 256) return f(std::integral_constant<int, 256>{});
-    return f(std::integral_constant<int, 128>{});
-}
-
 template <typename T>
 static bool rows_in_vectors(const RowOutput<T> &o, int columns)
 {
@@ -808,19 +794,21 @@ template <typename T, bool B_MN>
 static int multiply_rows(const ai2b_dense *d, const PackedRows &a, const PackedRows &w, const unsigned char *ws, const RowOutput<T> &o, int inner, int columns, cudaStream_t st)
 {
     constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
-    return with_columns<T>(columns_of_tile(d->dtype, columns), [&](auto bn) {
+    const tc::Tile tile = tc::best_tile(PLANES, d->rows, d->groups - 1, columns, 1, inner, sm_count());
+    return tc::with_tile<PLANES == 1 ? 256 : 128>(tile, [&](auto bn, auto pair) {
         constexpr int BN = decltype(bn)::value;
+        constexpr bool PAIR = decltype(pair)::value;
         tc::Operands ops{};
         int rc = map_rows(&ops.a, d->dtype, a, ws, d->rows, 1, tc::BM);
-        if (rc == AI2B_OK) rc = map_rows(&ops.b, d->dtype, w, ws, d->outer, d->groups, B_MN ? 64 : BN);
+        if (rc == AI2B_OK) rc = map_rows(&ops.b, d->dtype, w, ws, d->outer, d->groups, B_MN ? 64 : tile.b_rows());
         if (rc == AI2B_OK) rc = tc::flag_address(&ops.gave_up);
         if (rc != AI2B_OK) return rc;
         ops.a_stack = 1;
         ops.b_stack = d->groups;
         ops.is_bf16 = d->dtype != AI2B_F16;
-        const RowItems<BN> items{{d->d_offsets, d->groups, tc::BM, d->rows}, (columns + BN - 1) / BN, inner};
+        const RowItems<BN> items{{d->d_offsets, d->groups, tile.rows(), d->rows}, (columns + BN - 1) / BN, inner};
         const RowOut<T> out{o, columns, d->groups, rows_in_vectors(o, columns), common_alignment(o.bias) >= 16};
-        return tc::launch<PLANES, BN, false, B_MN>(ops, items, out, ((d->rows + tc::BM - 1) / tc::BM + d->groups) * items.column_tiles, st);
+        return tc::launch<PLANES, BN, PAIR, false, B_MN>(ops, items, out, ((d->rows + tile.rows() - 1) / tile.rows() + d->groups) * items.column_tiles, st);
     });
 }
 
@@ -828,8 +816,9 @@ template <typename T>
 static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const unsigned char *ws, float *part, cudaStream_t st)
 {
     constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
-    return with_columns<T>(columns_of_tile(d->dtype, d->inner), [&](auto bn) {
+    return tc::with_tile<PLANES == 1 ? 256 : 128>(p.weight_tile, [&](auto bn, auto pair) {
         constexpr int BN = decltype(bn)::value;
+        constexpr bool PAIR = decltype(pair)::value;
         tc::Operands ops{};
         int rc = map_rows(&ops.a, d->dtype, p.gz, ws, d->rows, 1, 64);
         if (rc == AI2B_OK) rc = map_rows(&ops.b, d->dtype, p.x, ws, d->rows, 1, 64);
@@ -837,9 +826,10 @@ static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const uns
         if (rc != AI2B_OK) return rc;
         ops.a_stack = ops.b_stack = 1;
         ops.is_bf16 = d->dtype != AI2B_F16;
-        const WeightItems<BN> items{{d->d_offsets, d->groups, p.weight_height, d->rows}, (d->outer + tc::BM - 1) / tc::BM, (d->inner + BN - 1) / BN, d->outer};
+        const int tile_rows = p.weight_tile.rows();
+        const WeightItems<BN> items{{d->d_offsets, d->groups, p.weight_height, d->rows}, tile_rows, (d->outer + tile_rows - 1) / tile_rows, (d->inner + BN - 1) / BN, d->outer};
         const WeightOut out{part, d->inner, d->outer, d->inner % 4 == 0};
-        return tc::launch<PLANES, BN, true, true>(ops, items, out, slab_bound(d->rows, p.weight_height, d->groups) * items.row_tiles * items.column_tiles, st);
+        return tc::launch<PLANES, BN, PAIR, true, true>(ops, items, out, slab_bound(d->rows, p.weight_height, d->groups) * items.row_tiles * items.column_tiles, st);
     });
 }
 

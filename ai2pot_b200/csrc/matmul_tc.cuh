@@ -4,6 +4,11 @@
 // tcgen05.mma into one of two accumulators in TMEM, the other warps take finished accumulators out and hand them to an epilogue while
 // the next tile is being multiplied. Tiles are 128 x BN, 64 of the summed index per stage.
 //
+// An SM takes in about 45 bytes a cycle from L2 (measured: 10 blocks of 128 x 128 as fast per stage as 148), and a stage of a 128 x 256 tile has 96
+// for every cycle of its products. With PAIR two neighbouring blocks (a cluster) share a tile of 256 rows: each holds its 128 rows of A, half
+// of B's tile and the accumulators of its rows, and one thread of the first issues the products of both (cta_group::2). That is 64 bytes
+// a cycle for 256 x 256.
+//
 // Operands are 16-bit matrices in memory with 16-byte aligned rows, read in the direction that they lie in: an operand whose rows run
 // along the summed index is K-major, one whose rows run along the tile's own index is MN-major (the tensor core takes both), so no
 // operand is transposed.
@@ -37,40 +42,80 @@ constexpr int WAIT_LIMIT = 1 << 20;
 __device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void barrier_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void barrier_expect(unsigned bar, unsigned bytes)
+// The same place in the shared memory of the pair's first block
+__device__ __forceinline__ unsigned in_first_block(unsigned address)
 {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+    unsigned d;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(d) : "r"(address));
+    return d;
 }
-__device__ __forceinline__ void barrier_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// (remote: an address in the cluster's shared memory)
+__device__ __forceinline__ void barrier_expect(unsigned remote, unsigned bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(remote), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(unsigned remote) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory"); }
 __device__ __forceinline__ bool barrier_try(unsigned bar, unsigned parity)
 {
     unsigned done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool barrier_wait(unsigned bar, unsigned parity)
+__device__ __forceinline__ bool barrier_wait_alone(unsigned bar, unsigned parity)
 {
-    bool ok = false;
-    for (int i = 0; i < WAIT_LIMIT && !ok; i++) ok = barrier_try(bar, parity);
-    return __all_sync(FULL_MASK, ok);      // whole warps wait, and go on or give up together
+    for (int i = 0; i < WAIT_LIMIT; i++)
+        if (barrier_try(bar, parity)) return true;
+    return false;
+}
+// Whole warps wait, and go on or give up together
+__device__ __forceinline__ bool barrier_wait(unsigned bar, unsigned parity) { return __all_sync(FULL_MASK, barrier_wait_alone(bar, parity)); }
+// True in one lane of the warp. (The compiler then knows that one thread issues what follows; of `lane == 0` it does not, and wraps every tensor-core
+// instruction and copy into a loop over the lanes.)
+__device__ __forceinline__ bool elect_one()
+{
+    unsigned p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Into this block's shared memory; the bytes are counted at a barrier of either block of the pair
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, int x, int y, int z, unsigned bar)
 {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z),
-                 "r"(bar)
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+                     "r"(x), "r"(y), "r"(z), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+                     "r"(z), "r"(bar)
+                     : "memory");
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool accumulate)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                 "r"((unsigned)accumulate)
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                     "r"((unsigned)accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                     "r"((unsigned)accumulate)
+                     : "memory");
 }
+// Arrives, once the products issued so far are done, at the barrier of every block that takes part
+template <bool PAIR>
 __device__ __forceinline__ void commit(unsigned bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tmem_load32(float (&v)[32], unsigned addr)
 {
@@ -93,9 +138,9 @@ __device__ __forceinline__ unsigned long long tile_descriptor(unsigned address, 
 }
 
 // Instruction descriptor: float accumulator, operands both bfloat16 or both half
-__host__ __device__ constexpr unsigned instruction_descriptor(bool is_bf16, bool a_mn, bool b_mn, int n)
+__host__ __device__ constexpr unsigned instruction_descriptor(bool is_bf16, bool a_mn, bool b_mn, int m, int n)
 {
-    return 1u << 4 | (is_bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (unsigned)(n >> 3) << 17 | (unsigned)(BM >> 4) << 24;
+    return 1u << 4 | (is_bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (unsigned)(n >> 3) << 17 | (unsigned)(m >> 4) << 24;
 }
 
 // ---- a tile of work -------------------------------------------------------------------------------------------------------
@@ -106,11 +151,14 @@ struct Item {
     int k_begin, k_end;           // range of the summed index; k_begin == k_end: the sums are zero
     long long row, row_end;       // rows and first column of the result
     int col, batch;
+    int mirror_from;              // results that are their own transpose: tiles from this column on are stored twice
 };
 
-template <int PLANES, int BN>
+template <int PLANES, int BN, bool PAIR>
 struct Shape {
-    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;      // one plane
+    static constexpr int BLOCKS = PAIR ? 2 : 1;                                      // that share a tile
+    static constexpr int B_ROWS = BN / BLOCKS;                                       // of B's tile in one block
+    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2;           // one plane
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
     static constexpr bool CAREFUL = PLANES > 1;
     // Sixteen epilogue warps: an activation with its slope is a chain of some 40 dependent instructions, and two warps per scheduler left it
@@ -130,13 +178,13 @@ struct Shape {
 };
 
 // A plane's tile in a stage: K-major one box of 64 x rows, MN-major a box of 64 x 64 for every 64 rows of the tile
-template <bool MN>
+template <bool PAIR, bool MN>
 __device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap *map, int rows, int at, int k, int batch, unsigned bar)
 {
     if constexpr (MN) {
-        for (int c = 0; c < rows; c += 64) tma_load(dst + c * BK * 2, map, at + c, k, batch, bar);
+        for (int c = 0; c < rows; c += 64) tma_load<PAIR>(dst + c * BK * 2, map, at + c, k, batch, bar);
     } else {
-        tma_load(dst, map, k, at, batch, bar);
+        tma_load<PAIR>(dst, map, k, at, batch, bar);
     }
 }
 
@@ -150,118 +198,171 @@ struct Operands {
 // Items::prepare(table), by all threads, may leave something in shared memory; Items::get(table, t, item), by whole warps, gives tile t, false after
 // the last one. (table is NULL, and nothing was prepared, where there is no room for it.) Out takes 32 x 32 sums at a time, in shared memory:
 // out.load(ahead, item, first row, first column, lane) reads what it needs of memory, out(item, first row, first column, sums, lane, ahead) stores.
-template <int PLANES, int BN, bool A_MN, bool B_MN, typename Items, typename Out>
-__global__ void __launch_bounds__(Shape<PLANES, BN>::THREADS, 1) product_kernel(const __grid_constant__ Operands ops, const __grid_constant__ Items items, const __grid_constant__ Out out)
+template <int PLANES, int BN, bool PAIR, bool A_MN, bool B_MN, typename Items, typename Out>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLANES, BN, PAIR>::THREADS, 1) product_kernel(const __grid_constant__ Operands ops, const __grid_constant__ Items items, const __grid_constant__ Out out)
 {
-    using S = Shape<PLANES, BN>;
+    using S = Shape<PLANES, BN, PAIR>;
     extern __shared__ unsigned char smem_raw[];
     const unsigned raw = smem_address(smem_raw), base = (raw + 1023) & ~1023u;
     unsigned char *smem = smem_raw + (base - raw);
     float *staging = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE_BYTES);
     const unsigned bars = base + S::STAGES * S::STAGE_BYTES + S::STAGING_BYTES;
-    const unsigned full = bars, empty = bars + 8 * STAGE_LIMIT, done = empty + 8 * STAGE_LIMIT, taken = done + 16, drained = taken + 16;
-    unsigned *tmem_slot = reinterpret_cast<unsigned *>(smem + (drained + 8 - base));
+    const unsigned full = bars, empty = bars + 8 * STAGE_LIMIT, done = empty + 8 * STAGE_LIMIT, taken = done + 16, drained = taken + 16, tail = drained + 8;
+    unsigned *tmem_slot = reinterpret_cast<unsigned *>(smem + (tail + 8 - base));
     int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
     int *table = S::TABLE ? reinterpret_cast<int *>(smem + (bars + 1024 - base)) : nullptr;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(FULL_MASK, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the same in every lane, and known to be)
     constexpr int TMEM_COLUMNS = S::TMEM_COLUMNS;
+    const int rank = PAIR ? blockIdx.x & 1 : 0;                 // in the pair: blocks 2 i and 2 i + 1
+    const long long first_tile = blockIdx.x / S::BLOCKS, tile_step = gridDim.x / S::BLOCKS;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) {
-            barrier_init(full + 8 * s, 1);
+            barrier_init(full + 8 * s, S::BLOCKS);              // (the first block's)
             barrier_init(empty + 8 * s, 1);
         }
         for (int b = 0; b < 2; b++) {
             barrier_init(done + 8 * b, 1);
-            barrier_init(taken + 8 * b, S::EPILOGUE_WARPS);
+            barrier_init(taken + 8 * b, S::BLOCKS * S::EPILOGUE_WARPS);      // (the first block's)
         }
         barrier_init(drained, 1);
+        barrier_init(tail, 1);
         *stopped = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(TMEM_COLUMNS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(TMEM_COLUMNS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(TMEM_COLUMNS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();      // both blocks' barriers are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = *tmem_slot;
     chain_wait();
     chain_release();
     if (S::TABLE) items.prepare(table);
 
+    const unsigned full_of_pair = PAIR ? in_first_block(full) : full, taken_of_pair = PAIR ? in_first_block(taken) : taken;
+    // Where the summed index runs over rows of memory in both operands, what follows k_end may belong to another network and hold NaN: it is
+    // zeroed in both, up to the 16 rows of the last step.
+    constexpr bool ZERO_TAIL = A_MN && B_MN;
+    auto ragged = [](int left) { return ZERO_TAIL && left < BK && (left & 15) != 0; };
+    auto zero_tail = [&](unsigned stage, int left) {
+        const int rows = (16 - (left & 15)) * 8;      // in pieces of 16 bytes: a row is 128 whole bytes whatever the swizzle
+        for (int i = lane; i < rows; i += 32) {
+            const unsigned at = (left + (i >> 3)) * 128 + (i & 7) * 16;
+            for (int c = 0; c < PLANES * (BM + S::B_ROWS) / 64; c++)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + c * BK * 128 + at), "r"(0) : "memory");
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
+    };
+
     bool ok = true;
     unsigned issued = 0;                 // stages that the producer has started
     if (warp == 0) {
         Item it;
-        for (long long t = blockIdx.x; ok && items.get(table, t, it); t += gridDim.x) {
-            for (int k = it.k_begin; ok && k < it.k_end; k += BK, issued++) {
-                const unsigned s = issued % S::STAGES, round = issued / S::STAGES;
-                ok = round == 0 || barrier_wait(empty + 8 * s, (round - 1) & 1);
-                if (!ok) break;
-                if (lane == 0) {
-                    barrier_expect(full + 8 * s, S::STAGE_BYTES);
+        for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
+            const int a_at = it.a_at + rank * BM, b_at = it.b_at + rank * S::B_ROWS;
+            const int stages = it.k_end > it.k_begin ? (it.k_end - it.k_begin + BK - 1) / BK : 0;
+            // one thread by itself: votes and barriers of the warp would cost more than the copies' issue
+            if (elect_one()) {
+                for (int i = 0; i < stages; i++) {
+                    const unsigned n = issued + i, s = n % S::STAGES, round = n / S::STAGES;
+                    const int k = it.k_begin + i * BK;
+                    ok = round == 0 || barrier_wait_alone(empty + 8 * s, (round - 1) & 1);
+                    if (!ok) break;
+                    // a pair's ragged stage is announced by the warp that has zeroed its end
+                    const bool local = PAIR && ragged(it.k_end - k);
+                    const unsigned bar = local ? tail : full_of_pair + 8 * s;
+                    barrier_expect(bar, S::STAGE_BYTES);
                     const unsigned dst = base + s * S::STAGE_BYTES;
 #pragma unroll
                     for (int p = 0; p < PLANES; p++) {
-                        load_tile<A_MN>(dst + p * S::A_BYTES, &ops.a, BM, it.a_at, k, it.a_batch + p * ops.a_stack, full + 8 * s);
-                        load_tile<B_MN>(dst + PLANES * S::A_BYTES + p * S::B_BYTES, &ops.b, BN, it.b_at, k, it.b_batch + p * ops.b_stack, full + 8 * s);
+                        load_tile<PAIR, A_MN>(dst + p * S::A_BYTES, &ops.a, BM, a_at, k, it.a_batch + p * ops.a_stack, bar);
+                        load_tile<PAIR, B_MN>(dst + PLANES * S::A_BYTES + p * S::B_BYTES, &ops.b, S::B_ROWS, b_at, k, it.b_batch + p * ops.b_stack, bar);
                     }
                 }
-                __syncwarp();
             }
+            ok = __all_sync(FULL_MASK, ok);
+            issued += stages;      // (after a wait that ran out this counts stages that never came: the waits for them end as well)
         }
     } else if (warp == 1) {
-        const unsigned idesc = instruction_descriptor(ops.is_bf16, A_MN, B_MN, BN);
+        const unsigned idesc = instruction_descriptor(ops.is_bf16, A_MN, B_MN, BM * S::BLOCKS, BN);
         Item it;
-        unsigned used = 0, sets = 0;          // sets of accumulators begun
-        for (long long t = blockIdx.x; ok && items.get(table, t, it); t += gridDim.x) {
+        unsigned used = 0, sets = 0, tails = 0;          // stages and sets of accumulators begun, ragged stages
+        for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
             for (int k0 = it.k_begin; ok && k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end) {
                 const unsigned set = sets & 1, d = tmem + set * S::ACCUMULATORS * BN;
-                if (sets >= 2) ok = barrier_wait(taken + 8 * set, ((sets >> 1) - 1) & 1);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int k = k0; k < it.k_end && (!S::CAREFUL || k < k0 + S::CHUNK); k += BK, used++) {
-                    const unsigned s = used % S::STAGES;
-                    ok = barrier_wait(full + 8 * s, (used / S::STAGES) & 1);
+                if (rank == 0) {
+                    if (sets >= 2) ok = barrier_wait(taken + 8 * set, ((sets >> 1) - 1) & 1);
                     if (!ok) break;
-                    const unsigned a = base + s * S::STAGE_BYTES, b = a + PLANES * S::A_BYTES;
-                    const int left = it.k_end - k, steps = left >= BK ? BK / 16 : (left + 15) / 16;
-                    if constexpr (A_MN && B_MN) {
-                        // The summed index runs over rows of memory, and what follows k_end may belong to another network: it may hold NaN, so
-                        // it is zeroed in both operands up to the 16 rows of the last step. A row is 128 whole bytes whatever the swizzle.
-                        if (left < steps * 16) {
-                            for (int i = lane; i < (steps * 16 - left) * 8; i += 32) {
-                                const unsigned at = (left + (i >> 3)) * 128 + (i & 7) * 16;
-                                for (int c = 0; c < PLANES * (BM + BN) / 64; c++)
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a + c * BK * 128 + at), "r"(0) : "memory");
-                            }
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
-                        }
-                    }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (lane == 0) {
-                        for (int step = 0; step < steps; step++) {
-                            // 16 of the summed index: 32 bytes along a K-major row, 16 rows of an MN-major tile
-                            const unsigned a_step = step * (A_MN ? 16 * 128 : 32), b_step = step * (B_MN ? 16 * 128 : 32);
-                            const bool more = k > k0 || step > 0;
-#pragma unroll
-                            for (int order = PLANES - 1; order >= 0; order--) {      // small pieces first
-#pragma unroll
-                                for (int pa = 0; pa <= order; pa++)
-                                    mma(order > 0 ? d + BN : d, tile_descriptor(a + pa * S::A_BYTES + a_step, BK * 128),
-                                        tile_descriptor(b + (order - pa) * S::B_BYTES + b_step, BK * 128), idesc, order == 0 ? more : more || order < PLANES - 1 || pa > 0);
-                            }
-                        }
-                        commit(empty + 8 * s);
-                    }
-                    __syncwarp();
                 }
+                const int end = S::CAREFUL && it.k_end - k0 > S::CHUNK ? k0 + S::CHUNK : it.k_end;
+                const int stages = (end - k0 + BK - 1) / BK, whole = ragged(end - k0 - (stages - 1) * BK) ? stages - 1 : stages;
+                auto multiply = [&](unsigned stage, int step, bool more) {
+                    const unsigned a = stage, b = stage + PLANES * S::A_BYTES;
+                    // 16 of the summed index: 32 bytes along a K-major row, 16 rows of an MN-major tile
+                    const unsigned a_step = step * (A_MN ? 16 * 128 : 32), b_step = step * (B_MN ? 16 * 128 : 32);
+#pragma unroll
+                    for (int order = PLANES - 1; order >= 0; order--) {      // small pieces first
+#pragma unroll
+                        for (int pa = 0; pa <= order; pa++)
+                            mma<PAIR>(order > 0 ? d + BN : d, tile_descriptor(a + pa * S::A_BYTES + a_step, BK * 128),
+                                      tile_descriptor(b + (order - pa) * S::B_BYTES + b_step, BK * 128), idesc, order == 0 ? more : more || order < PLANES - 1 || pa > 0);
+                    }
+                };
+                if (rank == 0 && elect_one()) {
+                    for (int i = 0; i < whole; i++) {
+                        const unsigned n = used + i, s = n % S::STAGES, stage = base + s * S::STAGE_BYTES;
+                        ok = barrier_wait_alone(full + 8 * s, (n / S::STAGES) & 1);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const int left = end - k0 - i * BK;
+                        if (left > BK - 16) {
+#pragma unroll
+                            for (int step = 0; step < BK / 16; step++) multiply(stage, step, i > 0 || step > 0);
+                        } else {
+                            for (int step = 0; step * 16 < left; step++) multiply(stage, step, i > 0 || step > 0);
+                        }
+                        commit<PAIR>(empty + 8 * s);
+                    }
+                }
+                ok = __all_sync(FULL_MASK, ok);
                 if (!ok) break;
-                if (lane == 0) commit(done + 8 * set);
+                if (whole < stages) {
+                    const unsigned n = used + whole, s = n % S::STAGES, stage = base + s * S::STAGE_BYTES;
+                    const int left = end - k0 - whole * BK;
+                    if constexpr (PAIR) {
+                        ok = barrier_wait(tail, tails++ & 1);
+                        if (!ok) break;
+                        zero_tail(stage, left);
+                        if (lane == 0) barrier_arrive(full_of_pair + 8 * s);
+                        __syncwarp();
+                    }
+                    if (rank == 0) {
+                        ok = barrier_wait(full + 8 * s, (n / S::STAGES) & 1);
+                        if (!ok) break;
+                        if constexpr (!PAIR) zero_tail(stage, left);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (elect_one()) {
+                            for (int step = 0; step * 16 < left; step++) multiply(stage, step, whole > 0 || step > 0);
+                            commit<PAIR>(empty + 8 * s);
+                        }
+                        __syncwarp();
+                    }
+                }
+                used += stages;
+                if (!ok) break;
+                if (rank == 0 && elect_one()) commit<PAIR>(done + 8 * set);
                 __syncwarp();
                 sets++;
             }
@@ -281,8 +382,8 @@ __global__ void __launch_bounds__(Shape<PLANES, BN>::THREADS, 1) product_kernel(
             out(it, row, col, mine, lane, ahead);
             __syncwarp();
         };
-        for (long long t = blockIdx.x; ok && items.get(table, t, it); t += gridDim.x) {
-            const long long row = it.row + 32 * quarter;
+        for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
+            const long long row = it.row + rank * BM + 32 * quarter;
             constexpr int PARTS = (BN + 32 * S::SHARES - 1) / (32 * S::SHARES);
             float sum[S::CAREFUL ? PARTS : 1][32];
             if constexpr (S::CAREFUL) {
@@ -305,7 +406,7 @@ __global__ void __launch_bounds__(Shape<PLANES, BN>::THREADS, 1) product_kernel(
                         for (int j = 0; j < 32; j++) sum[i][j] += v[j] + low[j];
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    if (lane == 0) barrier_arrive(taken + 8 * (sets & 1));
+                    if (lane == 0) barrier_arrive(taken_of_pair + 8 * (sets & 1));
                 }
                 if (!ok) break;
 #pragma unroll
@@ -342,7 +443,7 @@ __global__ void __launch_bounds__(Shape<PLANES, BN>::THREADS, 1) product_kernel(
                 }
                 if (sums) {
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    if (lane == 0) barrier_arrive(taken + 8 * set);
+                    if (lane == 0) barrier_arrive(taken_of_pair + 8 * set);
                     sets++;
                 }
             }
@@ -356,16 +457,20 @@ __global__ void __launch_bounds__(Shape<PLANES, BN>::THREADS, 1) product_kernel(
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (*stopped) {
-        // copies in flight write into this block's shared memory, products into its TMEM
-        if (warp == 0)
+        // copies in flight write into the blocks' shared memory, products into their TMEM; the first block knows of both
+        if (warp == 0 && rank == 0)
             for (unsigned i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; i++) barrier_wait(full + 8 * (i % S::STAGES), (i / S::STAGES) & 1);
-        if (warp == 1) {
-            if (lane == 0) commit(drained);
+        if (warp == 1 && rank == 0) {
+            if (elect_one()) commit<PAIR>(drained);
             barrier_wait(drained, 0);
         }
         __syncthreads();
     }
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS) : "memory");
+    if constexpr (PAIR) cluster_sync();      // nothing is on its way to a block that leaves
+    if (warp == 1) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLUMNS) : "memory");
+    }
 }
 
 // What an epilogue reads of a warp's 32 x 32 sums: columns [4 i, 4 i + 4) of row r
@@ -379,17 +484,94 @@ __device__ __forceinline__ float4 staged(const float *mine, int r, int i) { retu
 int flag_address(int **flag);
 int make_map(CUtensorMap *map, const void *p, bool is_bf16, long long columns, long long rows, long long batch, long long row_stride, long long batch_stride, int box_rows);
 
-template <int PLANES, int BN, bool A_MN, bool B_MN, typename Items, typename Out>
+// Pairs of blocks that the current device holds at once (kept with the kernel's other set-up; neighbouring SMs may be missing)
+template <typename Kern>
+int resident_pairs(KernelSetup &ks, Kern kern, int threads, size_t smem, int *pairs)
+{
+    int dev = 0;
+    AI2B_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> guard(ks.mu);
+    if (dev < MAX_DEVICES && ks.per_sm[dev] > 0) {
+        *pairs = ks.per_sm[dev];
+        return AI2B_OK;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)sm_count() / 2 * 2);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    int n = 0;
+    AI2B_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+    *pairs = n > 0 ? n : 1;
+    if (dev < MAX_DEVICES) ks.per_sm[dev] = *pairs;
+    return AI2B_OK;
+}
+
+template <int PLANES, int BN, bool PAIR, bool A_MN, bool B_MN, typename Items, typename Out>
 int launch(const Operands &ops, const Items &items, const Out &out, long long tiles, cudaStream_t st)
 {
-    using S = Shape<PLANES, BN>;
-    auto kern = product_kernel<PLANES, BN, A_MN, B_MN, Items, Out>;
+    using S = Shape<PLANES, BN, PAIR>;
+    auto kern = product_kernel<PLANES, BN, PAIR, A_MN, B_MN, Items, Out>;
     static KernelSetup ks;
     const int rc = kernel_setup(ks, kern, S::SMEM);
     if (rc != AI2B_OK) return rc;
-    const int sms = sm_count();
-    AI2B_CUDA(launch_chained(kern, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(S::THREADS), S::SMEM, st, ops, items, out));
+    int units = sm_count();
+    if constexpr (PAIR) {
+        const int rc2 = resident_pairs(ks, kern, S::THREADS, S::SMEM, &units);
+        if (rc2 != AI2B_OK) return rc2;
+    }
+    AI2B_CUDA(launch_chained(kern, dim3((unsigned)(tiles < units ? tiles : units) * S::BLOCKS), dim3(S::THREADS), S::SMEM, st, ops, items, out));
     return AI2B_OK;
+}
+
+// The tile of a product: BN columns, 128 rows or, by a pair of blocks, 256
+struct Tile {
+    int columns;
+    bool pair;
+    int rows() const { return pair ? 2 * BM : BM; }
+    int b_rows() const { return pair ? columns / 2 : columns; }      // box of a K-major B
+};
+
+// What the products of `rows` x `columns` results (`matrices` of them; `edges` more tiles of rows that are not full) would take in tiles of
+// one kind, in cycles: per stage the longer of its products and of its copies at 45 bytes a cycle; a tile's last stage and its epilogue (22 cycles a
+// column) are not overlapped by another of the same block.
+inline double tile_cost(Tile t, int planes, long long rows, long long edges, long long columns, long long matrices, long long inner, int sms)
+{
+    const int terms = planes * (planes + 1) / 2;
+    const double products = 2.0 * t.columns * terms, copies = planes * 128.0 * (BM + t.b_rows()) / 45.0;
+    const double tiles = (double)matrices * (double)((rows + t.rows() - 1) / t.rows() + edges) * (double)((columns + t.columns - 1) / t.columns);
+    const double waves = (double)(long long)((tiles + sms / (t.pair ? 2 : 1) - 1) / (sms / (t.pair ? 2 : 1)));
+    const double stages = (double)((inner + BK - 1) / BK), epilogue = 22.0 * t.columns;
+    const double tile = stages * (products > copies ? products : copies);
+    return waves * (tile > epilogue ? tile : epilogue) + epilogue + 1500.0;
+}
+// The kind that takes least. (Planes need two accumulators for each of two tiles: 128 columns at most.)
+inline Tile best_tile(int planes, long long rows, long long edges, long long columns, long long matrices, long long inner, int sms)
+{
+    Tile best{64, false};
+    double least = 1e300;
+    for (int bn = 64; bn <= (planes > 1 ? 128 : 256); bn *= 2)
+        for (int pair = 0; pair < 2; pair++) {
+            if (pair && bn == 64) continue;
+            const Tile t{bn, pair != 0};
+            const double cost = tile_cost(t, planes, rows, edges, columns, matrices, inner, sms);
+            if (cost < least) {
+                least = cost;
+                best = t;
+            }
+        }
+    return best;
+}
+
+// f(integral_constant<BN>, integral_constant<PAIR>) of a tile; LARGEST: 128 or 256 columns
+template <int LARGEST, typename F>
+int with_tile(Tile t, F &&f)
+{
+    using std::integral_constant;
+    if (t.columns == 64) return f(integral_constant<int, 64>{}, std::false_type{});
+    if constexpr (LARGEST == 256) {
+        if (t.columns == 256) return t.pair ? f(integral_constant<int, 256>{}, std::true_type{}) : f(integral_constant<int, 256>{}, std::false_type{});
+    }
+    return t.pair ? f(integral_constant<int, 128>{}, std::true_type{}) : f(integral_constant<int, 128>{}, std::false_type{});
 }
 
 }  // namespace tc

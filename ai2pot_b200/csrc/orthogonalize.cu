@@ -107,35 +107,36 @@ __global__ void __launch_bounds__(256) normalise_halves_kernel(f16 *__restrict__
     }
 }
 
-// 128 x BN tiles of a batch of products; with `symmetric` (BN = 128) those on and above the diagonal
+// tile_rows x BN tiles of a batch of products; with `symmetric` those that reach the diagonal or lie above it
 template <int BN>
 struct BatchItems {
-    int row_tiles, column_tiles, inner, rows, batch;
+    int tile_rows, row_tiles, column_tiles, inner, rows, batch;
     bool symmetric;
+    int tiles() const { return symmetric ? before(row_tiles) : row_tiles * column_tiles; }
+    // tiles of the rows of tiles before r
+    __host__ __device__ __forceinline__ int before(int r) const { return r * column_tiles - tile_rows / BN * (r * (r - 1) / 2); }
     __device__ __forceinline__ void prepare(int *) const {}
     __device__ __forceinline__ bool get(const int *, long long t, tc::Item &it) const
     {
-        const int per = symmetric ? row_tiles * (row_tiles + 1) / 2 : row_tiles * column_tiles;
+        const int per = symmetric ? before(row_tiles) : row_tiles * column_tiles;
         const int b = (int)(t / per);
         if (b >= batch) return false;
         int i = (int)(t - (long long)b * per), r = 0;
         if (symmetric) {
-            // rows of the triangle hold row_tiles, row_tiles - 1, ... tiles
-            const float n = row_tiles + 0.5f;
-            r = max(0, (int)(n - sqrtf(fmaxf(n * n - 2.f * i, 0.f))) - 1);
-            while (i >= (r + 1) * row_tiles - (r + 1) * r / 2) r++;
-            i = i - (r * row_tiles - r * (r - 1) / 2) + r;
+            while (before(r + 1) <= i) r++;
+            i += tile_rows / BN * r - before(r);
         } else {
             r = i / column_tiles;
             i -= r * column_tiles;
         }
-        it.a_at = r * tc::BM;
+        it.a_at = r * tile_rows;
         it.b_at = it.col = i * BN;
         it.a_batch = it.b_batch = it.batch = b;
         it.k_begin = 0;
         it.k_end = inner;
         it.row = it.a_at;
         it.row_end = rows;
+        it.mirror_from = symmetric ? it.a_at + tile_rows : 0x7fffffff;
         return true;
     }
 };
@@ -149,7 +150,7 @@ struct BatchOut {
     T *result;
     int columns, rows;
     long long stride;                     // of the halves' rows, a multiple of 8
-    bool symmetric;
+    bool symmetric;                       // (host) the result is its own transpose
 
     struct Ahead {};
     __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
@@ -165,7 +166,7 @@ struct BatchOut {
                 store(s, matrix + row + r, col, columns);
             }
         }
-        if (symmetric && it.a_at != it.b_at) {
+        if (it.col >= it.mirror_from) {
             // rows and columns exchanged: eight rows of the sums make up a piece of a row
             const int r0 = lane % 4 * 8;
 #pragma unroll 1
@@ -260,22 +261,22 @@ struct Halves {
 template <int PLANES, bool A_MN, bool B_MN, typename Out>
 static int product_tc(const Halves &a, const Halves &b, const Out &out, int inner, int batch, cudaStream_t st)
 {
-    // float: two planes of 128 columns fill the accumulators. Symmetric products want square tiles.
-    auto go = [&](auto bn) {
+    tc::Tile tile = tc::best_tile(PLANES, out.rows, 0, out.columns, batch, inner, sm_count());
+    // half of a symmetric result is not multiplied: tiles are square, or two to a square
+    if (out.symmetric && tile.columns > tile.rows()) tile.columns = tile.rows();
+    if (out.symmetric && tile.columns < 128) tile.columns = 128;
+    return tc::with_tile<PLANES == 1 ? 256 : 128>(tile, [&](auto bn, auto pair) {
         constexpr int BN = decltype(bn)::value;
+        constexpr bool PAIR = decltype(pair)::value;
         tc::Operands ops{};
         int rc = tc::make_map(&ops.a, a.hi, false, a.columns, a.rows, (long long)batch * PLANES, a.stride, a.rows * a.stride, A_MN ? 64 : tc::BM);
-        if (rc == AI2B_OK) rc = tc::make_map(&ops.b, b.hi, false, b.columns, b.rows, (long long)batch * PLANES, b.stride, b.rows * b.stride, B_MN ? 64 : BN);
+        if (rc == AI2B_OK) rc = tc::make_map(&ops.b, b.hi, false, b.columns, b.rows, (long long)batch * PLANES, b.stride, b.rows * b.stride, B_MN ? 64 : tile.b_rows());
         if (rc == AI2B_OK) rc = tc::flag_address(&ops.gave_up);
         if (rc != AI2B_OK) return rc;
         ops.a_stack = ops.b_stack = batch;
-        const BatchItems<BN> items{(out.rows + tc::BM - 1) / tc::BM, (out.columns + BN - 1) / BN, inner, out.rows, batch, out.symmetric};
-        const long long per = out.symmetric ? (long long)items.row_tiles * (items.row_tiles + 1) / 2 : (long long)items.row_tiles * items.column_tiles;
-        return tc::launch<PLANES, BN, A_MN, B_MN>(ops, items, out, per * batch, st);
-    };
-    if constexpr (PLANES == 1)
-        if (!out.symmetric && (long long)batch * ((out.rows + 127) / 128) * ((out.columns + 255) / 256) >= sm_count()) return go(std::integral_constant<int, 256>{});
-    return go(std::integral_constant<int, 128>{});
+        const BatchItems<BN> items{tile.rows(), (out.rows + tile.rows() - 1) / tile.rows(), (out.columns + BN - 1) / BN, inner, out.rows, batch, out.symmetric};
+        return tc::launch<PLANES, BN, PAIR, A_MN, B_MN>(ops, items, out, (long long)items.tiles() * batch, st);
+    });
 }
 
 // The iteration on halves: PLANES of them are multiplied
