@@ -4,8 +4,8 @@
 // tcgen05.mma into one of two accumulators in TMEM, the other warps take finished accumulators out and hand them to an epilogue while
 // the next tile is being multiplied. Tiles are 128 x BN, 64 of the summed index per stage.
 //
-// An SM takes in about 45 bytes a cycle from L2 (measured: 10 blocks of 128 x 128 as fast per stage as 148), and a stage of a 128 x 256 tile has 96
-// for every cycle of its products. With PAIR two neighbouring blocks (a cluster) share a tile of 256 rows: each holds its 128 rows of A, half
+// An SM takes in about 58 bytes a cycle from L2 (measured: a stage of 24 KB in 410 cycles, whatever the products), and a stage of a 128 x 256 tile
+// has 96 for every cycle of its products. With PAIR two neighbouring blocks (a cluster) share a tile of 256 rows: each holds its 128 rows of A, half
 // of B's tile and the accumulators of its rows, and one thread of the first issues the products of both (cta_group::2). That is 64 bytes
 // a cycle for 256 x 256.
 //
@@ -207,8 +207,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
     unsigned char *smem = smem_raw + (base - raw);
     float *staging = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE_BYTES);
     const unsigned bars = base + S::STAGES * S::STAGE_BYTES + S::STAGING_BYTES;
-    const unsigned full = bars, empty = bars + 8 * STAGE_LIMIT, done = empty + 8 * STAGE_LIMIT, taken = done + 16, drained = taken + 16, tail = drained + 8;
-    unsigned *tmem_slot = reinterpret_cast<unsigned *>(smem + (tail + 8 - base));
+    const unsigned full = bars, empty = bars + 8 * STAGE_LIMIT, done = empty + 8 * STAGE_LIMIT, taken = done + 16, drained = taken + 16, tail = drained + 8;      // tail: one per stage
+    unsigned *tmem_slot = reinterpret_cast<unsigned *>(smem + (tail + 8 * STAGE_LIMIT - base));
     int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
     int *table = S::TABLE ? reinterpret_cast<int *>(smem + (bars + 1024 - base)) : nullptr;
     const int warp = __shfl_sync(FULL_MASK, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the same in every lane, and known to be)
@@ -220,13 +220,13 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
         for (int s = 0; s < S::STAGES; s++) {
             barrier_init(full + 8 * s, S::BLOCKS);              // (the first block's)
             barrier_init(empty + 8 * s, 1);
+            barrier_init(tail + 8 * s, 1);
         }
         for (int b = 0; b < 2; b++) {
             barrier_init(done + 8 * b, 1);
             barrier_init(taken + 8 * b, S::BLOCKS * S::EPILOGUE_WARPS);      // (the first block's)
         }
         barrier_init(drained, 1);
-        barrier_init(tail, 1);
         *stopped = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
@@ -266,9 +266,9 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
     };
 
     bool ok = true;
-    unsigned issued = 0;                 // stages that the producer has started
     if (warp == 0) {
         Item it;
+        unsigned issued = 0;             // stages started
         for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
             const int a_at = it.a_at + rank * BM, b_at = it.b_at + rank * S::B_ROWS;
             const int stages = it.k_end > it.k_begin ? (it.k_end - it.k_begin + BK - 1) / BK : 0;
@@ -281,7 +281,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                     if (!ok) break;
                     // a pair's ragged stage is announced by the warp that has zeroed its end
                     const bool local = PAIR && ragged(it.k_end - k);
-                    const unsigned bar = local ? tail : full_of_pair + 8 * s;
+                    const unsigned bar = (local ? tail : full_of_pair) + 8 * s;
                     barrier_expect(bar, S::STAGE_BYTES);
                     const unsigned dst = base + s * S::STAGE_BYTES;
 #pragma unroll
@@ -292,12 +292,12 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                 }
             }
             ok = __all_sync(FULL_MASK, ok);
-            issued += stages;      // (after a wait that ran out this counts stages that never came: the waits for them end as well)
+            issued += stages;
         }
     } else if (warp == 1) {
         const unsigned idesc = instruction_descriptor(ops.is_bf16, A_MN, B_MN, BM * S::BLOCKS, BN);
         Item it;
-        unsigned used = 0, sets = 0, tails = 0;          // stages and sets of accumulators begun, ragged stages
+        unsigned used = 0, sets = 0, tails = 0;          // stages and sets of accumulators begun; a bit per stage, turned over by its ragged uses
         for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
             for (int k0 = it.k_begin; ok && k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end) {
                 const unsigned set = sets & 1, d = tmem + set * S::ACCUMULATORS * BN;
@@ -342,8 +342,9 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                     const unsigned n = used + whole, s = n % S::STAGES, stage = base + s * S::STAGE_BYTES;
                     const int left = end - k0 - whole * BK;
                     if constexpr (PAIR) {
-                        ok = barrier_wait(tail, tails++ & 1);
+                        ok = barrier_wait(tail + 8 * s, tails >> s & 1);
                         if (!ok) break;
+                        tails ^= 1u << s;
                         zero_tail(stage, left);
                         if (lane == 0) barrier_arrive(full_of_pair + 8 * s);
                         __syncwarp();
@@ -457,13 +458,13 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (*stopped) {
-        // copies in flight write into the blocks' shared memory, products into their TMEM; the first block knows of both
-        if (warp == 0 && rank == 0)
-            for (unsigned i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; i++) barrier_wait(full + 8 * (i % S::STAGES), (i / S::STAGES) & 1);
+        // Products write into the blocks' TMEM: wait for those issued. Copies write into this block's shared memory, and which of them are under way
+        // only the barriers know that ran out: they take microseconds, so they are given milliseconds.
         if (warp == 1 && rank == 0) {
             if (elect_one()) commit<PAIR>(drained);
             barrier_wait(drained, 0);
         }
+        for (int i = 0; i < 20; i++) __nanosleep(500000);
         __syncthreads();
     }
     if constexpr (PAIR) cluster_sync();      // nothing is on its way to a block that leaves
@@ -532,12 +533,12 @@ struct Tile {
 };
 
 // What the products of `rows` x `columns` results (`matrices` of them; `edges` more tiles of rows that are not full) would take in tiles of
-// one kind, in cycles: per stage the longer of its products and of its copies at 45 bytes a cycle; a tile's last stage and its epilogue (22 cycles a
+// one kind, in cycles: per stage the longer of its products and of its copies at 58 bytes a cycle; a tile's last stage and its epilogue (22 cycles a
 // column) are not overlapped by another of the same block.
 inline double tile_cost(Tile t, int planes, long long rows, long long edges, long long columns, long long matrices, long long inner, int sms)
 {
     const int terms = planes * (planes + 1) / 2;
-    const double products = 2.0 * t.columns * terms, copies = planes * 128.0 * (BM + t.b_rows()) / 45.0;
+    const double products = 2.0 * t.columns * terms, copies = planes * 128.0 * (BM + t.b_rows()) / 58.0;
     const double tiles = (double)matrices * (double)((rows + t.rows() - 1) / t.rows() + edges) * (double)((columns + t.columns - 1) / t.columns);
     const double waves = (double)(long long)((tiles + sms / (t.pair ? 2 : 1) - 1) / (sms / (t.pair ? 2 : 1)));
     const double stages = (double)((inner + BK - 1) / BK), epilogue = 22.0 * t.columns;

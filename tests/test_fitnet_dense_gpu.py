@@ -76,6 +76,19 @@ def test_larger_layers(sizes, inner, outer, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_short_ragged_groups(dtype):
+    """Groups of a few stages whose rows do not fill the last one, between long ones, in layers whose tiles are the largest: their ragged
+    stages follow each other within the stages that are in flight."""
+    sizes = [3000, 189, 23, 76, 5, 2100, 100, 63, 65, 1, 129, 2500, 47, 190, 33]
+    offsets = torch.tensor([0] + sizes).cumsum(0).int().cuda()
+    t, gy = make(sum(sizes), len(sizes), 1024, 1024, dtype)
+    first = check(t, "gelu", offsets, gy)
+    for _ in range(5):
+        again = run(t, "gelu", offsets, gy)
+        assert all(torch.equal(first[key], again[key]) for key in first)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_many_groups(dtype):
     sizes = [(37 * e) % 19 for e in range(1024)]
     offsets = torch.tensor([0] + sizes).cumsum(0).int().cuda()
