@@ -4,8 +4,8 @@
 //   gz = gy * s;  gx = gz W_e;  gW_e = sum over the rows of e of gz^T x;  gb_e = sum of gz;  gresidual = gy
 //   rows after the last group belong to no network: y, gx and gresidual are zero there
 //
-// Products are accumulated in float. gz is rounded to the element type of x where it becomes a factor of the products (their other factor
-// has that type already); gb adds it unrounded. s lies between -0.13 and 1.13, so that 16-bit layers of either type keep it as a half, which
+// Products are accumulated in float. gz is rounded to the element type of x where it becomes a factor on the tensor cores (whose two factors have
+// one type); gb adds it unrounded, and so do the products on the FMA pipes. s lies between -0.13 and 1.13, so that 16-bit layers of either type keep it as a half, which
 // has the more digits: rounding it costs nothing next to gz in bfloat16 (errors of gx against 64 bits: 0.0030 with s in bfloat16, 0.0024).
 // The sums over rows (gW, gb) are cut into slabs of rows whose partial sums are added in a fixed order: no atomics.
 #include "fitnet.cuh"
@@ -204,8 +204,8 @@ __device__ __forceinline__ void store_row_element(const RowOutput<T> &o, long lo
 }
 
 // Rows of every group times the group's matrix: w[group][.][.] has strides sj (column of the output) and sk (summed index).
-template <typename T>
-__global__ void __launch_bounds__(256) rows_fma_kernel(const T *__restrict__ x, long long x_stride, const T *__restrict__ w, long long w_size, long long w_sj, long long w_sk,
+template <typename T, typename A>
+__global__ void __launch_bounds__(256) rows_fma_kernel(const A *__restrict__ x, long long x_stride, const T *__restrict__ w, long long w_size, long long w_sj, long long w_sk,
                                                        const int *__restrict__ offsets, int groups, long long rows, int inner, int columns, RowOutput<T> o)
 {
     __shared__ float As[FK][FT + 4], Bs[FK][FT + 4];
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(256) rows_fma_kernel(const T *__restrict__ x, 
     const int j0 = blockIdx.y * FT, ti = threadIdx.x / 16, tj = threadIdx.x % 16;
     float acc[4][4] = {};
     if (tile.group < groups)
-        fma_tile(acc, Operand<T>{x, x_stride, 1, tile.end, inner}, Operand<T>{w + tile.group * w_size, w_sj, w_sk, columns, inner}, tile.begin, j0, As, Bs);
+        fma_tile(acc, Operand<A>{x, x_stride, 1, tile.end, inner}, Operand<T>{w + tile.group * w_size, w_sj, w_sk, columns, inner}, tile.begin, j0, As, Bs);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -229,9 +229,45 @@ __global__ void __launch_bounds__(256) rows_fma_kernel(const T *__restrict__ x, 
         }
 }
 
+// A few rows (a step of one atom): bound by reading the matrix once. A warp takes C columns of R rows of one group, its lanes N neighbouring
+// elements of the summed index each; the sums of the lanes are exchanged so that each lane finishes one of the R C results.
+template <typename T, int N, int R, int C>
+__global__ void __launch_bounds__(256) thin_rows_kernel(const T *__restrict__ x, long long x_stride, const T *__restrict__ w, const int *__restrict__ offsets, int groups, long long rows,
+                                                        int inner, int columns, RowOutput<T> o)
+{
+    chain_wait();
+    chain_release();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j0 = (blockIdx.x * 8 + warp) * C;
+    if (j0 >= columns) return;
+    const RowTile tile = find_tile(offsets, groups, rows, R, blockIdx.y);
+    if (tile.group < 0) return;
+    float acc[R * C] = {};
+    if (tile.group < groups) {
+        const T *wg = w + (long long)tile.group * columns * inner;
+        for (int k = lane * N; k < inner; k += 32 * N) {
+            Pack<T, N> wv[C], xv[R];
+#pragma unroll
+            for (int c = 0; c < C; c++) wv[c] = *reinterpret_cast<const Pack<T, N> *>(wg + (long long)min(j0 + c, columns - 1) * inner + k);
+#pragma unroll
+            for (int r = 0; r < R; r++) xv[r] = *reinterpret_cast<const Pack<T, N> *>(x + min(tile.begin + r, tile.end - 1) * x_stride + k);
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int n = 0; n < N; n++) acc[r * C + c] = fmaf(to_float(xv[r].v[n]), to_float(wv[c].v[n]), acc[r * C + c]);
+        }
+    }
+    const float z = warp_xreduce<float, R * C>(acc, lane);      // lane l: result l / (32 / (R C))
+    const int i = lane / (32 / (R * C)), r = i / C, col = j0 + i % C;
+    if (lane % (32 / (R * C)) != 0 || tile.begin + r >= tile.end || col >= columns) return;
+    if (tile.group < groups) store_row_element(o, tile.begin + r, col, columns, tile.group, z);
+    else o.out[(tile.begin + r) * columns + col] = from_float<T>(0.f);
+}
+
 // Partial sums of gz^T x over slabs of rows: part[slab][outer][inner]
-template <typename T>
-__global__ void __launch_bounds__(256) weight_fma_kernel(const T *__restrict__ gz, long long gz_stride, const T *__restrict__ x, long long x_stride, const int *__restrict__ offsets,
+template <typename T, typename A>
+__global__ void __launch_bounds__(256) weight_fma_kernel(const A *__restrict__ gz, long long gz_stride, const T *__restrict__ x, long long x_stride, const int *__restrict__ offsets,
                                                          int groups, long long rows, int height, int outer, int inner, float *__restrict__ part)
 {
     __shared__ float As[FK][FT + 4], Bs[FK][FT + 4];
@@ -242,7 +278,7 @@ __global__ void __launch_bounds__(256) weight_fma_kernel(const T *__restrict__ g
     const int i0 = blockIdx.y * FT, j0 = blockIdx.z * FT, ti = threadIdx.x / 16, tj = threadIdx.x % 16;
     float acc[4][4] = {};
     const long long n = tile.end - tile.begin;
-    fma_tile(acc, Operand<T>{gz + tile.begin * gz_stride, 1, gz_stride, outer, n}, Operand<T>{x + tile.begin * x_stride, 1, x_stride, inner, n}, i0, j0, As, Bs);
+    fma_tile(acc, Operand<A>{gz + tile.begin * gz_stride, 1, gz_stride, outer, n}, Operand<T>{x + tile.begin * x_stride, 1, x_stride, inner, n}, i0, j0, As, Bs);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -273,30 +309,47 @@ __device__ __forceinline__ void split(float v, bf16 (&out)[PLANES])
 
 // Operand of a tensor-core product from rows that it cannot read as they are: 16-bit rows with other alignment are copied, floats
 // are cut into PLANES planes. out[plane][row][stride], `count` rows of `columns` each.
-template <typename T, int PLANES>
+// A thread takes eight columns of a row; N: how many of them one access reads.
+template <typename T, int PLANES, int N>
 __global__ void __launch_bounds__(256) pack_kernel(void *__restrict__ out, long long stride, const T *__restrict__ in, long long in_stride, long long count, int columns)
 {
+    using P = std::conditional_t<PLANES == 1, T, bf16>;
     chain_wait();
     chain_release();
-    const long long total = count * columns;
+    const int per_row = (int)(stride / 8);
+    const long long total = count * per_row;
+    const bool narrow = total <= 0xffffffffLL;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / columns;
-        const int c = (int)(i - r * columns);
-        const T v = in[r * in_stride + c];
-        if constexpr (PLANES == 1) {
-            reinterpret_cast<T *>(out)[r * stride + c] = v;
-        } else {
-            bf16 piece[PLANES];
-            split(to_float(v), piece);
+        const long long r = row_of(i, per_row, narrow);
+        const int c = (int)(i - r * per_row) * 8;
+        T v[8];
 #pragma unroll
-            for (int p = 0; p < PLANES; p++) reinterpret_cast<bf16 *>(out)[(p * count + r) * stride + c] = piece[p];
+        for (int j = 0; j < 8; j += N) {
+            Pack<T, N> p{};
+            if (c + j < columns) p = *reinterpret_cast<const Pack<T, N> *>(in + r * in_stride + c + j);
+#pragma unroll
+            for (int n = 0; n < N; n++) v[j + n] = p.v[n];
         }
+        Pack<P, 8> pieces[PLANES];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (PLANES == 1) {
+                pieces[0].v[j] = v[j];
+            } else {
+                bf16 piece[PLANES];
+                split(to_float(v[j]), piece);
+#pragma unroll
+                for (int p = 0; p < PLANES; p++) pieces[p].v[j] = piece[p];
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PLANES; p++) *reinterpret_cast<Pack<P, 8> *>(reinterpret_cast<P *>(out) + (p * count + r) * stride + c) = pieces[p];
     }
 }
 
-// gz = gy * slope (as PLANES planes of pieces where that is not 1), gresidual = gy (zero after the last group), and the column sums of
+// gz = gy * slope, of type G (as PLANES planes of pieces where that is not 1), gresidual = gy (zero after the last group), and the column sums of
 // gz over each slab: part[slab][outer]. A lane takes N columns, a warp every eighth row of the slab, four of them in flight.
-template <typename T, int PLANES, int N>
+template <typename T, typename G, int PLANES, int N>
 __global__ void __launch_bounds__(256) slope_kernel(void *__restrict__ gz, long long gz_stride, T *__restrict__ gresidual, float *__restrict__ part, const T *__restrict__ gy,
                                                     long long gy_stride, const Slope<T> *__restrict__ slope, const int *__restrict__ offsets, int groups, long long rows, int height,
                                                     int outer)
@@ -335,14 +388,14 @@ __global__ void __launch_bounds__(256) slope_kernel(void *__restrict__ gz, long 
                     continue;
                 }
                 if (gresidual) *reinterpret_cast<Pack<T, N> *>(gresidual + r * outer + col) = g[u];
-                Pack<std::conditional_t<PLANES == 1, T, bf16>, N> pieces[PLANES];
+                Pack<G, N> pieces[PLANES];
 #pragma unroll
                 for (int n = 0; n < N; n++) {
                     float v = to_float(g[u].v[n]);
                     if (slope) v *= to_float(s[u].v[n]);
                     sum[n] += v;
                     if constexpr (PLANES == 1) {
-                        pieces[0].v[n] = from_float<T>(v);
+                        pieces[0].v[n] = from_float<G>(v);
                     } else {
                         bf16 piece[PLANES];
                         split(v, piece);
@@ -521,39 +574,70 @@ struct RowOut {
     struct Ahead {
         Pack<T, N> residual, bias;      // of the first pass
     };
-    __device__ __forceinline__ Pack<T, N> read(const T *p, int col, bool whole) const
-    {
-        Pack<T, N> v;
-        if (whole) {
-            v = *reinterpret_cast<const Pack<T, N> *>(p);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; j++) v.v[j] = col + j < columns ? p[j] : from_float<T>(0.f);
-        }
-        return v;
-    }
     __device__ __forceinline__ void load(Ahead &a, const tc::Item &it, long long row, int col0, int lane) const
     {
         const int col = col0 + lane % LANES * N;
-        if (it.batch >= groups || col >= columns) return;
-        if (o.bias) a.bias = read(o.bias + (long long)it.batch * columns + col, col, vectors && bias_vectors);
-        if (o.residual) a.residual = read(o.residual + min(row + lane / LANES, it.row_end - 1) * o.residual_stride + col, col, vectors);
+        if (!vectors || it.batch >= groups || col >= columns) return;
+        if (o.bias) {
+            const T *p = o.bias + (long long)it.batch * columns + col;
+            if (bias_vectors) {
+                a.bias = *reinterpret_cast<const Pack<T, N> *>(p);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++) a.bias.v[j] = p[j];
+            }
+        }
+        if (o.residual) a.residual = *reinterpret_cast<const Pack<T, N> *>(o.residual + min(row + lane / LANES, it.row_end - 1) * o.residual_stride + col);
+    }
+
+    // Two results of one column: sums and bias in z, what comes out in value and slope
+    template <int ACT, bool SLOPE>
+    static __device__ __forceinline__ Activated2 finish(float2 z)
+    {
+        if constexpr (sizeof(T) == 2) {
+            return activate2<ACT, SLOPE>(z);
+        } else {
+            const Activated a = activate<ACT>(z.x), b = activate<ACT>(z.y);
+            return Activated2{make_float2(a.value, b.value), make_float2(a.slope, b.slope)};
+        }
     }
 
     template <int ACT, bool SLOPE>
     __device__ __forceinline__ void apply(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &ahead) const
     {
-        const int i0 = lane % LANES * N, col = col0 + i0, n = min(N, columns - col);
-        if (n <= 0) return;
         const bool kept = it.batch < groups, add = o.residual && kept;
+        const int last = (int)min((long long)32, it.row_end - row);
+        if (!vectors) {
+            // a column a lane, two rows at a time (eight columns a lane, element by element, took 6 us more for each 1157 x 97 results)
+            const int col = col0 + lane;
+            if (col >= columns) return;
+            const float bias = o.bias && kept ? to_float(o.bias[(long long)it.batch * columns + col]) : 0.f;
+#pragma unroll 2
+            for (int r = 0; r < last; r += 2) {
+                const long long at = row + r;
+                const bool two = r + 1 < last;
+                float2 z;
+                z.x = mine[32 * r + 4 * ((lane / 4) ^ (r & 7)) + lane % 4] + bias;
+                z.y = mine[32 * (r + 1) + 4 * ((lane / 4) ^ ((r + 1) & 7)) + lane % 4] + bias;
+                Activated2 a = finish<ACT, SLOPE>(z);
+                if (add) {
+                    a.value.x += to_float(o.residual[at * o.residual_stride + col]);
+                    if (two) a.value.y += to_float(o.residual[(at + 1) * o.residual_stride + col]);
+                }
+                o.out[at * columns + col] = from_float<T>(a.value.x);
+                if (two) o.out[(at + 1) * columns + col] = from_float<T>(a.value.y);
+                if constexpr (SLOPE) {
+                    o.slope[at * columns + col] = from_float<Slope<T>>(a.slope.x);
+                    if (two) o.slope[(at + 1) * columns + col] = from_float<Slope<T>>(a.slope.y);
+                }
+            }
+            return;
+        }
+        const int i0 = lane % LANES * N, col = col0 + i0;
+        if (col >= columns) return;
         float2 bias[N / 2];
 #pragma unroll
-        for (int j = 0; j < N / 2; j++) {
-            if constexpr (sizeof(T) == 4) bias[j] = make_float2(ahead.bias.v[2 * j], ahead.bias.v[2 * j + 1]);
-            else bias[j] = widen(ahead.bias.v[2 * j], ahead.bias.v[2 * j + 1]);
-            if (!o.bias || !kept) bias[j] = both(0.f);
-        }
-        const int last = (int)min((long long)32, it.row_end - row);
+        for (int j = 0; j < N / 2; j++) bias[j] = o.bias && kept ? make_float2(to_float(ahead.bias.v[2 * j]), to_float(ahead.bias.v[2 * j + 1])) : both(0.f);
         T *py = o.out + (row + lane / LANES) * columns + col;
         Slope<T> *ps = SLOPE ? o.slope + (row + lane / LANES) * columns + col : nullptr;
         Pack<T, N> residual, next = ahead.residual;
@@ -561,7 +645,7 @@ struct RowOut {
 #pragma unroll 1
         for (int r = lane / LANES; r < last; r += ROWS, py += ROWS * (long long)columns) {
             residual = next;
-            if (add && r + ROWS < last) next = read(o.residual + (row + r + ROWS) * o.residual_stride + col, col, vectors);
+            if (add && r + ROWS < last) next = *reinterpret_cast<const Pack<T, N> *>(o.residual + (row + r + ROWS) * o.residual_stride + col);
             float2 z[N / 2];
 #pragma unroll
             for (int j = 0; j < N; j += 4) {
@@ -573,31 +657,24 @@ struct RowOut {
             Pack<Slope<T>, N> slope;
 #pragma unroll
             for (int j = 0; j < N; j += 2) {
-                if constexpr (sizeof(T) == 4) {
-                    const Activated a = activate<ACT>(z[j / 2].x), b = activate<ACT>(z[j / 2].y);
-                    y.v[j] = add ? a.value + residual.v[j] : a.value;
-                    y.v[j + 1] = add ? b.value + residual.v[j + 1] : b.value;
-                    slope.v[j] = a.slope;
-                    slope.v[j + 1] = b.slope;
-                } else {
-                    Activated2 a = activate2<ACT, SLOPE>(z[j / 2]);
+                Activated2 a = finish<ACT, SLOPE>(z[j / 2]);
+                if constexpr (sizeof(T) == 2) {
                     if (add) a.value = add2(a.value, widen(residual.v[j], residual.v[j + 1]));
                     narrow(&y.v[j], a.value);
                     if constexpr (SLOPE) narrow(&slope.v[j], a.slope);
+                } else {
+                    if (add) a.value = add2(a.value, make_float2(residual.v[j], residual.v[j + 1]));
+                    y.v[j] = a.value.x;
+                    y.v[j + 1] = a.value.y;
+                    slope.v[j] = a.slope.x;
+                    slope.v[j + 1] = a.slope.y;
                 }
             }
-            if (vectors) {
-                *reinterpret_cast<Pack<T, N> *>(py) = y;
-                if constexpr (SLOPE) *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (j < n) {
-                        py[j] = y.v[j];
-                        if constexpr (SLOPE) ps[j] = slope.v[j];
-                    }
+            *reinterpret_cast<Pack<T, N> *>(py) = y;
+            if constexpr (SLOPE) {
+                *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
+                ps += ROWS * (long long)columns;
             }
-            if constexpr (SLOPE) ps += ROWS * (long long)columns;
         }
     }
     template <int ACT>
@@ -684,8 +761,20 @@ static long long slab_bound(long long rows, int height, int groups) { return (ro
 static int planes_of(int dtype) { return dtype == AI2B_F32 ? 3 : 1; }
 static long long padded(long long n) { return (n + 7) / 8 * 8; }
 
-// The FMA pipes take what is small: there the tensor-core kernel's set-up (barriers, TMEM, tensor maps) is not made up for.
-static bool on_tensor_cores(const ai2b_dense *d) { return d->rows > 0 && (double)d->rows * d->inner * d->outer >= 4e6; }
+// Which products go to the tensor cores, from times of both (us, FMA pipes / tensor cores). Forward, float (two launches more, to cut the
+// operands into planes): 216 x 64 x 64 7.5 / 8.9, 216 x 128 x 128 12.3 / 9.8, 216 x 1024 x 1024 79 / 24, 65536 x 32 x 32 19.6 / 18.9. 16 bits: 216 x 64 x 64
+// 9.6 / 4.3; operands that have to be copied: 216 x 20 x 30 5.9 / 7.6, 1157 x 131 x 97 20 / 12. Gradient, float: 32 x 1024 x 64 15.5 / 19.4,
+// 216 x 20 x 30 25 / 22; 16 bits: 32 x 32 x 32 13.1 / 13.7, 216 x 64 x 64 37 / 16.
+static bool forward_on_tensor_cores(const ai2b_dense *d)
+{
+    if (d->rows <= 16) return false;
+    if (d->dtype == AI2B_F32) return d->inner > 64;
+    return d->inner > 32 || common_alignment(d->d_x, d->d_weight, 2 * d->x_stride, 2LL * d->inner) >= 16;
+}
+static bool backward_on_tensor_cores(const ai2b_dense *d) { return d->rows > (d->dtype == AI2B_F32 ? 64 : 32); }
+
+// Up to 16 rows the matrix is read by warps as it lies (1 x 1024 x 1024 in bfloat16: 81 us in 64 x 64 tiles)
+static bool thin(const ai2b_dense *d) { return d->rows <= 16; }
 
 // An operand of a tensor-core product: rows as they lie in memory, or a packed copy of them in the workspace
 struct PackedRows {
@@ -711,7 +800,7 @@ struct ForwardPlan {
 static ForwardPlan plan_forward(const ai2b_dense *d)
 {
     ForwardPlan p{};
-    p.tensor = on_tensor_cores(d);
+    p.tensor = forward_on_tensor_cores(d);
     if (p.tensor) {
         p.x = packed_rows(d->dtype, d->d_x, d->x_stride, d->rows, d->inner, &p.total);
         p.weight = packed_rows(d->dtype, d->d_weight, d->inner, (long long)d->groups * d->outer, d->inner, &p.total);
@@ -736,7 +825,7 @@ static int slope_vectors(const ai2b_dense *d)
 static BackwardPlan plan_backward(const ai2b_dense *d)
 {
     BackwardPlan p{};
-    p.tensor = on_tensor_cores(d);
+    p.tensor = backward_on_tensor_cores(d);
     p.slopes = d->activation != AI2B_ACT_NONE;
     if (p.tensor) {
         // tiles of a slab of 2048 rows, as many slabs as there are
@@ -756,7 +845,7 @@ static BackwardPlan plan_backward(const ai2b_dense *d)
         p.gz = PackedRows{d->d_gy, d->gy_stride, d->rows, d->outer, false, 0};
         if (p.slopes) {
             p.gz.copy = true;
-            p.total += round256(element_bytes(d->dtype) * (size_t)d->rows * padded(d->outer));
+            p.total += round256(sizeof(float) * (size_t)d->rows * padded(d->outer));
         }
     }
     p.weight_part = p.total;
@@ -770,10 +859,15 @@ template <typename T>
 static int pack(const PackedRows &p, unsigned char *ws, cudaStream_t st)
 {
     if (!p.copy) return AI2B_OK;
-    const long long blocks = (p.count * p.columns + 255) / 256;
-    constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
-    AI2B_CUDA(launch_chained(pack_kernel<T, PLANES>, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st, (void *)(ws + p.at), p.stride(), (const T *)p.from,
-                             p.from_stride, p.count, (int)p.columns));
+    const long long blocks = (p.count * p.stride() / 8 + 255) / 256;
+    constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1, N = std::is_same<T, float>::value ? 4 : 1;
+    // (16-bit rows are copied because they are not aligned, float ones because they are float)
+    const bool vectors = N > 1 && common_alignment(p.from, 4 * p.from_stride, 4 * p.columns) >= 16;
+    auto go = [&](auto kern) {
+        return launch_chained(kern, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st, (void *)(ws + p.at), p.stride(), (const T *)p.from, p.from_stride,
+                              p.count, (int)p.columns);
+    };
+    AI2B_CUDA(vectors ? go(pack_kernel<T, PLANES, N>) : go(pack_kernel<T, PLANES, 1>));
     return AI2B_OK;
 }
 
@@ -833,6 +927,26 @@ static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const uns
     });
 }
 
+template <typename T>
+static int thin_rows(const ai2b_dense *d, const RowOutput<T> &o, cudaStream_t st)
+{
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool vectors = common_alignment(d->d_x, d->d_weight, (long long)sizeof(T) * d->inner, (long long)sizeof(T) * (d->rows > 1 ? d->x_stride : 0)) >= 16;
+    auto go = [&](auto kern, int rows, int columns) {
+        const dim3 grid((d->outer + 8 * columns - 1) / (8 * columns), (unsigned)((d->rows + rows - 1) / rows + (d->d_offsets ? d->groups : 0)));
+        AI2B_CUDA(launch_chained(kern, grid, dim3(256), 0, st, (const T *)d->d_x, d->x_stride, (const T *)d->d_weight, d->d_offsets, d->groups, d->rows, d->inner, d->outer, o));
+        return (int)AI2B_OK;
+    };
+    // four columns a warp where there are enough for every SM
+    const bool many = d->outer >= 4 * 8 * sm_count();
+    if (d->rows == 1) {
+        if (vectors) return many ? go(thin_rows_kernel<T, N, 1, 4>, 1, 4) : go(thin_rows_kernel<T, N, 1, 1>, 1, 1);
+        return many ? go(thin_rows_kernel<T, 1, 1, 4>, 1, 4) : go(thin_rows_kernel<T, 1, 1, 1>, 1, 1);
+    }
+    if (vectors) return many ? go(thin_rows_kernel<T, N, 8, 4>, 8, 4) : go(thin_rows_kernel<T, N, 8, 1>, 8, 1);
+    return many ? go(thin_rows_kernel<T, 1, 8, 4>, 8, 4) : go(thin_rows_kernel<T, 1, 8, 1>, 8, 1);
+}
+
 static int check_dense(const ai2b_dense *d, const char *what)
 {
     AI2B_REQUIRE(d, AI2B_ERR_INVALID, "%s: NULL description", what);
@@ -882,8 +996,9 @@ extern "C" int ai2b_dense_forward(const ai2b_dense *d, void *stream)
             if (rc2 == AI2B_OK) rc2 = multiply_rows<T, false>(d, p.x, p.weight, ws, o, d->inner, d->outer, st);
             return rc2;
         }
+        if (thin(d)) return thin_rows(d, o, st);
         const dim3 grid((unsigned)((d->rows + FT - 1) / FT + d->groups), (d->outer + FT - 1) / FT);
-        AI2B_CUDA(launch_chained(rows_fma_kernel<T>, grid, dim3(256), 0, st, (const T *)d->d_x, d->x_stride, (const T *)d->d_weight, (long long)d->outer * d->inner,
+        AI2B_CUDA(launch_chained(rows_fma_kernel<T, T>, grid, dim3(256), 0, st, (const T *)d->d_x, d->x_stride, (const T *)d->d_weight, (long long)d->outer * d->inner,
                                  (long long)d->inner, 1LL, d->d_offsets, d->groups, d->rows, d->inner, d->outer, o));
         return (int)AI2B_OK;
     });
@@ -914,10 +1029,12 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
             };
             constexpr int N = 16 / (int)sizeof(T);
             if constexpr (std::is_same<T, float>::value)
-                if (p.tensor) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<float, 3, N>) : go(slope_kernel<float, 3, 1>));
-            if (!(std::is_same<T, float>::value && p.tensor)) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<T, 1, N>) : go(slope_kernel<T, 1, 1>));
+                if (p.tensor) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<float, bf16, 3, N>) : go(slope_kernel<float, bf16, 3, 1>));
+            if constexpr (!std::is_same<T, float>::value)
+                if (p.tensor) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<T, T, 1, N>) : go(slope_kernel<T, T, 1, 1>));
+            if (!p.tensor) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<T, float, 1, N>) : go(slope_kernel<T, float, 1, 1>));
         }
-        const T *gz = (const T *)(p.gz.copy ? ws + p.gz.at : d->d_gy);
+        const void *gz = p.gz.copy ? ws + p.gz.at : d->d_gy;      // (on the FMA pipes: float if made here, else gy)
         if (d->d_gx && d->rows > 0) {
             const RowOutput<T> o{(T *)d->d_gx, nullptr, nullptr, nullptr, 0, AI2B_ACT_NONE};
             if (p.tensor) {
@@ -926,8 +1043,11 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
                 if (rc2 != AI2B_OK) return rc2;
             } else {
                 const dim3 grid((unsigned)((d->rows + FT - 1) / FT + d->groups), (d->inner + FT - 1) / FT);
-                AI2B_CUDA(launch_chained(rows_fma_kernel<T>, grid, dim3(256), 0, st, gz, p.gz.stride(), (const T *)d->d_weight, (long long)d->outer * d->inner, 1LL,
-                                         (long long)d->inner, d->d_offsets, d->groups, d->rows, d->outer, d->inner, o));
+                auto go = [&](auto kern, auto *from) {
+                    return launch_chained(kern, grid, dim3(256), 0, st, from, p.gz.stride(), (const T *)d->d_weight, (long long)d->outer * d->inner, 1LL, (long long)d->inner,
+                                          d->d_offsets, d->groups, d->rows, d->outer, d->inner, o);
+                };
+                AI2B_CUDA(p.gz.copy ? go(rows_fma_kernel<T, float>, (const float *)gz) : go(rows_fma_kernel<T, T>, (const T *)gz));
             }
         }
         if (d->d_gweight) {
@@ -937,8 +1057,11 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
                 if (rc2 != AI2B_OK) return rc2;
             } else if (d->rows > 0) {
                 const dim3 grid((unsigned)slab_bound(d->rows, p.weight_height, d->groups), (d->outer + FT - 1) / FT, (d->inner + FT - 1) / FT);
-                AI2B_CUDA(launch_chained(weight_fma_kernel<T>, grid, dim3(256), 0, st, gz, p.gz.stride(), (const T *)d->d_x, d->x_stride, d->d_offsets, d->groups, d->rows,
-                                         p.weight_height, d->outer, d->inner, wpart));
+                auto go = [&](auto kern, auto *from) {
+                    return launch_chained(kern, grid, dim3(256), 0, st, from, p.gz.stride(), (const T *)d->d_x, d->x_stride, d->d_offsets, d->groups, d->rows, p.weight_height,
+                                          d->outer, d->inner, wpart);
+                };
+                AI2B_CUDA(p.gz.copy ? go(weight_fma_kernel<T, float>, (const float *)gz) : go(weight_fma_kernel<T, T>, (const T *)gz));
             }
         }
         if (d->d_gweight || d->d_gbias) {

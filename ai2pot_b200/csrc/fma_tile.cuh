@@ -6,7 +6,7 @@ namespace ai2b {
 
 // C[i][j] = sum_k A[i][k] B[j][k] for a 64 x 64 tile of C, 256 threads with 4 x 4 sums each. Any strides: what the tensor-core
 // kernels do not take comes here.
-constexpr int FT = 64, FK = 16;
+constexpr int FT = 64, FK = 32;
 
 template <typename T>
 struct Operand {
@@ -15,22 +15,44 @@ struct Operand {
     long long ni, nk;         // their extents
 };
 
+// This thread's eight elements of a 64 x 32 piece: neighbouring threads along the direction that is contiguous in memory
+template <typename T>
+__device__ __forceinline__ void fma_fetch(float (&v)[FT * FK / 256], const Operand<T> &o, long long i0, long long k0)
+{
+#pragma unroll
+    for (int u = 0; u < FT * FK / 256; u++) {
+        const int e = threadIdx.x + 256 * u, i = o.sk == 1 ? e / FK : e % FT, k = o.sk == 1 ? e % FK : e / FT;
+        v[u] = i0 + i < o.ni && k0 + k < o.nk ? to_float(o.p[(i0 + i) * o.si + (k0 + k) * o.sk]) : 0.f;
+    }
+}
+__device__ __forceinline__ void fma_put(float (*s)[FT + 4], const float (&v)[FT * FK / 256], bool k_contiguous)
+{
+#pragma unroll
+    for (int u = 0; u < FT * FK / 256; u++) {
+        const int e = threadIdx.x + 256 * u;
+        s[k_contiguous ? e % FK : e / FT][k_contiguous ? e / FK : e % FT] = v[u];
+    }
+}
+
+// The next piece is on its way from memory while this one is multiplied.
 template <typename TA, typename TB>
 __device__ __forceinline__ void fma_tile(float (&acc)[4][4], const Operand<TA> &A, const Operand<TB> &B, long long i0, long long j0, float (*As)[FT + 4], float (*Bs)[FT + 4])
 {
-    const int tid = threadIdx.x, ti = tid / 16, tj = tid % 16;
+    const int ti = threadIdx.x / 16, tj = threadIdx.x % 16;
+    float a_next[FT * FK / 256], b_next[FT * FK / 256];
+    if (A.nk > 0) {
+        fma_fetch(a_next, A, i0, 0);
+        fma_fetch(b_next, B, j0, 0);
+    }
     for (long long k0 = 0; k0 < A.nk; k0 += FK) {
-#pragma unroll
-        for (int u = 0; u < FT * FK / 256; u++) {
-            const int e = tid + 256 * u;
-            // neighbouring threads along the direction that is contiguous in memory
-            const int ia = A.sk == 1 ? e / FK : e % FT, ka = A.sk == 1 ? e % FK : e / FT;
-            const int jb = B.sk == 1 ? e / FK : e % FT, kb = B.sk == 1 ? e % FK : e / FT;
-            As[ka][ia] = i0 + ia < A.ni && k0 + ka < A.nk ? to_float(A.p[(i0 + ia) * A.si + (k0 + ka) * A.sk]) : 0.f;
-            Bs[kb][jb] = j0 + jb < B.ni && k0 + kb < B.nk ? to_float(B.p[(j0 + jb) * B.si + (k0 + kb) * B.sk]) : 0.f;
-        }
+        fma_put(As, a_next, A.sk == 1);
+        fma_put(Bs, b_next, B.sk == 1);
         __syncthreads();
-#pragma unroll
+        if (k0 + FK < A.nk) {
+            fma_fetch(a_next, A, i0, k0 + FK);
+            fma_fetch(b_next, B, j0, k0 + FK);
+        }
+#pragma unroll 8
         for (int k = 0; k < FK; k++) {
             const float4 a = *reinterpret_cast<const float4 *>(&As[k][4 * ti]), b = *reinterpret_cast<const float4 *>(&Bs[k][4 * tj]);
             const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};

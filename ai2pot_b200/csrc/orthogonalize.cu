@@ -40,14 +40,21 @@ __global__ void __launch_bounds__(256) norm_kernel(const T *__restrict__ g, long
     }
 }
 
+// 1 / (norm + eps) from the partial sums, the same in every thread of every block
+__device__ __forceinline__ double norm_scale(const double *part, int parts, double eps)
+{
+    const int lane = threadIdx.x & 31;
+    double sum = 0.0;
+    for (int i = lane; i < parts; i += 32) sum += part[i];
+    return 1.0 / (sqrt(warp_sum(sum)) + eps);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) normalise_kernel(float *__restrict__ x, const T *__restrict__ g, long long size, int parts, const double *__restrict__ part, double eps)
 {
     chain_wait();
     chain_release();
-    double sum = 0.0;
-    for (int i = 0; i < parts; i++) sum += part[blockIdx.y * NORM_BLOCKS + i];
-    const double scale = 1.0 / (sqrt(sum) + eps);
+    const double scale = norm_scale(part + blockIdx.y * NORM_BLOCKS, parts, eps);
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (long long)gridDim.x * blockDim.x)
         x[blockIdx.y * size + i] = (float)((double)to_float(g[blockIdx.y * size + i]) * scale);
 }
@@ -97,9 +104,7 @@ __global__ void __launch_bounds__(256) normalise_halves_kernel(f16 *__restrict__
 {
     chain_wait();
     chain_release();
-    double sum = 0.0;
-    for (int i = 0; i < parts; i++) sum += part[blockIdx.y * NORM_BLOCKS + i];
-    const double scale = 1.0 / (sqrt(sum) + eps);
+    const double scale = norm_scale(part + blockIdx.y * NORM_BLOCKS, parts, eps);
     const long long size = (long long)m * n;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (long long)gridDim.x * blockDim.x) {
         const long long r = row_of(i, n, size <= 0xffffffffLL), at = (blockIdx.y * (long long)m + r) * stride + (i - r * n);
