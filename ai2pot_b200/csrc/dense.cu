@@ -902,6 +902,11 @@ static int multiply_rows(const ai2b_dense *d, const PackedRows &a, const PackedR
         ops.is_bf16 = d->dtype != AI2B_F16;
         const RowItems<BN> items{{d->d_offsets, d->groups, tile.rows(), d->rows}, (columns + BN - 1) / BN, inner};
         const RowOut<T> out{o, columns, d->groups, rows_in_vectors(o, columns), common_alignment(o.bias) >= 16};
+        if (o.residual && out.vectors) {
+            rc = tc::make_prefetch_map(&ops.ahead, o.residual, d->dtype, columns, d->rows, o.residual_stride);
+            if (rc != AI2B_OK) return rc;
+            ops.ahead_columns = 128 / (int)sizeof(T);
+        }
         return tc::launch<PLANES, BN, PAIR, false, B_MN>(ops, items, out, ((d->rows + tile.rows() - 1) / tile.rows() + d->groups) * items.column_tiles, st);
     });
 }

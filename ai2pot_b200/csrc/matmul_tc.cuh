@@ -96,6 +96,11 @@ __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, i
                      : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap *map, int x, int y, int z)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 template <bool PAIR>
 __device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool accumulate)
 {
@@ -190,6 +195,8 @@ __device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap *map, 
 
 struct Operands {
     CUtensorMap a, b;
+    CUtensorMap ahead;            // what the epilogue reads of memory: brought to L2 when the tile's first stages are (columns of a box; 0: nothing)
+    int ahead_columns;
     int a_stack, b_stack;         // matrices in one plane of each operand
     int is_bf16;
     int *gave_up;                 // set by a wait that ran out
@@ -274,6 +281,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
             const int stages = it.k_end > it.k_begin ? (it.k_end - it.k_begin + BK - 1) / BK : 0;
             // one thread by itself: votes and barriers of the warp would cost more than the copies' issue
             if (elect_one()) {
+                for (int c = 0; ops.ahead_columns > 0 && stages > 0 && c < BN && it.col + c < out.columns; c += ops.ahead_columns)
+                    tma_prefetch(&ops.ahead, it.col + c, (int)it.row + rank * BM, 0);
                 for (int i = 0; i < stages; i++) {
                     const unsigned n = issued + i, s = n % S::STAGES, round = n / S::STAGES;
                     const int k = it.k_begin + i * BK;
@@ -484,6 +493,8 @@ __device__ __forceinline__ float4 staged(const float *mine, int r, int i) { retu
 // flag_address: where the current device's products report a wait that ran out
 int flag_address(int **flag);
 int make_map(CUtensorMap *map, const void *p, bool is_bf16, long long columns, long long rows, long long batch, long long row_stride, long long batch_stride, int box_rows);
+// The same for prefetches of a matrix of any element type: boxes of 128 bytes x 128 rows, no swizzle
+int make_prefetch_map(CUtensorMap *map, const void *p, int dtype, long long columns, long long rows, long long row_stride);
 
 // Pairs of blocks that the current device holds at once (kept with the kernel's other set-up; neighbouring SMs may be missing)
 template <typename Kern>

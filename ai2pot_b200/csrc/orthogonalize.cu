@@ -85,6 +85,137 @@ __global__ void __launch_bounds__(256) product_fma_kernel(T *__restrict__ out, f
         }
 }
 
+// ---- small matrices: the whole iteration in one block ----------------------------------------------------------------------------
+
+// The matrix, its Gram matrix and the polynomial stay in shared memory, S rows of L columns with S <= L (transposed on the way in and out where
+// m > n). A thread makes M x M results at a time. 3 x 30 x 20: 15 products as launches of their own took 56 us.
+constexpr int SMALL_THREADS = 512;
+constexpr size_t SMALL_BYTES = 200 * 1024;
+__host__ __device__ constexpr int odd(int n) { return n | 1; }      // row pitch: rows start in different banks
+static size_t small_bytes(int s, int l) { return sizeof(float) * ((size_t)s * odd(l) + 2 * (size_t)s * odd(s)); }
+
+// f(i, j, sums) for every M x M group of results C[i..][j..] = sum_k A[i][k] B[k][j], with element (k, j) of B at b[k * bk + j * bj]
+template <int M, typename F>
+__device__ __forceinline__ void small_product(int ni, int nj, int nk, const float *a, int pitch, const float *b, int bk, int bj, int first, int last, F &&f)
+{
+    const int groups_j = (nj + M - 1) / M;
+    for (int t = first; t < last; t += SMALL_THREADS) {
+        const int i0 = t / groups_j * M, j0 = t % groups_j * M;
+        const float *pa[M], *pb[M];
+#pragma unroll
+        for (int u = 0; u < M; u++) {
+            pa[u] = a + min(i0 + u, ni - 1) * pitch;
+            pb[u] = b + min(j0 + u, nj - 1) * bj;
+        }
+        float sum[M][M] = {};
+#pragma unroll 4
+        for (int k = 0; k < nk; k++) {
+            float av[M], bv[M];
+#pragma unroll
+            for (int u = 0; u < M; u++) {
+                av[u] = pa[u][k];
+                bv[u] = pb[u][k * bk];
+            }
+#pragma unroll
+            for (int u = 0; u < M; u++)
+#pragma unroll
+                for (int w = 0; w < M; w++) sum[u][w] = fmaf(av[u], bv[w], sum[u][w]);
+        }
+        f(i0, j0, sum);
+    }
+}
+
+template <typename T, int M>
+__global__ void __launch_bounds__(SMALL_THREADS) small_kernel(T *__restrict__ out, const T *__restrict__ g, int m, int n, int steps, float a, float b, float c, double eps)
+{
+    extern __shared__ float small_smem[];
+    __shared__ double sums[SMALL_THREADS / 32];
+    const bool wide = m <= n;
+    const int s = wide ? m : n, l = wide ? n : m, pl = odd(l), ps = odd(s), tid = threadIdx.x;
+    float *x = small_smem, *gram = x + s * pl, *poly = gram + s * ps;
+    chain_wait();
+    chain_release();
+    const T *mine = g + (long long)blockIdx.x * m * n;
+    double sum = 0.0;
+    for (int i = tid; i < m * n; i += SMALL_THREADS) {
+        const int r = i / n, q = i - r * n;
+        const float v = to_float(mine[i]);
+        x[wide ? r * pl + q : q * pl + r] = v;
+        sum += (double)v * v;
+    }
+    sum = warp_sum(sum);
+    if ((tid & 31) == 0) sums[tid >> 5] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < SMALL_THREADS / 32; w++) sum += sums[w];
+    const double scale = 1.0 / (sqrt(sum) + eps);
+    for (int i = tid; i < s * l; i += SMALL_THREADS) {
+        const int r = i / l, q = i - r * l;
+        x[r * pl + q] = (float)((double)x[r * pl + q] * scale);
+    }
+    __syncthreads();
+    const int square = ((s + M - 1) / M) * ((s + M - 1) / M), wide_groups = ((s + M - 1) / M) * ((l + M - 1) / M);
+    for (int step = 0; step < steps; step++) {
+        small_product<M>(s, s, l, x, pl, x, 1, pl, tid, square, [&](int i0, int j0, const float (&v)[M][M]) {
+#pragma unroll
+            for (int u = 0; u < M; u++)
+#pragma unroll
+                for (int w = 0; w < M; w++)
+                    if (i0 + u < s && j0 + w < s) gram[(i0 + u) * ps + j0 + w] = v[u][w];
+        });
+        __syncthreads();
+        small_product<M>(s, s, s, gram, ps, gram, ps, 1, tid, square, [&](int i0, int j0, const float (&v)[M][M]) {
+#pragma unroll
+            for (int u = 0; u < M; u++)
+#pragma unroll
+                for (int w = 0; w < M; w++)
+                    if (i0 + u < s && j0 + w < s) poly[(i0 + u) * ps + j0 + w] = fmaf(b, gram[(i0 + u) * ps + j0 + w], c * v[u][w]);
+        });
+        __syncthreads();
+        // x = a x + poly x, in place: a round's results are written after all of it has been read. Groups go down the columns first, so that a round
+        // is of whole columns, which no other round reads.
+        const int down = (s + M - 1) / M, per_round = SMALL_THREADS / down * down;
+        for (int t0 = 0; t0 < wide_groups; t0 += per_round) {
+            const int t = t0 + tid, i0 = t % down * M, j0 = t / down * M;
+            const bool in = tid < per_round && t < wide_groups;
+            float v[M][M] = {};
+            if (in) {
+#pragma unroll 4
+                for (int k = 0; k < s; k++) {
+                    float av[M], bv[M];
+#pragma unroll
+                    for (int u = 0; u < M; u++) {
+                        av[u] = poly[min(i0 + u, s - 1) * ps + k];
+                        bv[u] = x[k * pl + min(j0 + u, l - 1)];
+                    }
+#pragma unroll
+                    for (int u = 0; u < M; u++)
+#pragma unroll
+                        for (int w = 0; w < M; w++) v[u][w] = fmaf(av[u], bv[w], v[u][w]);
+                }
+#pragma unroll
+                for (int u = 0; u < M; u++)
+#pragma unroll
+                    for (int w = 0; w < M; w++) v[u][w] = fmaf(a, x[min(i0 + u, s - 1) * pl + min(j0 + w, l - 1)], v[u][w]);
+            }
+            __syncthreads();
+            if (in) {
+#pragma unroll
+                for (int u = 0; u < M; u++)
+#pragma unroll
+                    for (int w = 0; w < M; w++)
+                        if (i0 + u < s && j0 + w < l) x[(i0 + u) * pl + j0 + w] = v[u][w];
+            }
+        }
+        __syncthreads();
+    }
+    T *to = out + (long long)blockIdx.x * m * n;
+    for (int i = tid; i < m * n; i += SMALL_THREADS) {
+        const int r = i / n, q = i - r * n;
+        to[i] = from_float<T>(x[wide ? r * pl + q : q * pl + r]);
+    }
+}
+
 // ---- on the tensor cores ----------------------------------------------------------------------------------------------------
 
 // A number v is kept as halves of SCALE v: hi, and lo = what hi leaves. X has singular values of about one at most, so that its elements are
@@ -158,46 +289,70 @@ struct BatchOut {
     bool symmetric;                       // (host) the result is its own transpose
 
     struct Ahead {};
+    struct Added {
+        Pack<f16, 8> hi, lo;
+    };
     __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
     __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &) const
     {
         const int i0 = lane % 4 * 8, col = col0 + i0;
         const long long matrix = (long long)it.batch * rows;
+        // (two rows at a time on their way: more do not fit the registers)
         if (col < columns) {
 #pragma unroll 1
-            for (int r = lane / 4; r < 32 && row + r < it.row_end; r += 8) {
-                const float4 s0 = tc::staged(mine, r, i0 / 4), s1 = tc::staged(mine, r, i0 / 4 + 1);
-                const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-                store(s, matrix + row + r, col, columns);
+            for (int r = lane / 4; row + r < it.row_end && r < 32; r += 16) {
+                const bool two = row + r + 8 < it.row_end;
+                Added d0, d1;
+                read(d0, matrix + row + r, col);
+                if (two) read(d1, matrix + row + r + 8, col);
+                store_row(mine, r, i0, d0, matrix + row + r, col);
+                if (two) store_row(mine, r + 8, i0, d1, matrix + row + r + 8, col);
             }
         }
         if (it.col >= it.mirror_from) {
             // rows and columns exchanged: eight rows of the sums make up a piece of a row
             const int r0 = lane % 4 * 8;
+            if (row + r0 >= it.row_end) return;
 #pragma unroll 1
-            for (int c = lane / 4; c < 32 && col0 + c < columns; c += 8) {
-                if (row + r0 >= it.row_end) break;
-                float s[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) s[j] = mine[32 * (r0 + j) + 4 * ((c / 4) ^ ((r0 + j) & 7)) + c % 4];
-                store(s, matrix + col0 + c, (int)row + r0, columns);
+            for (int c = lane / 4; col0 + c < columns && c < 32; c += 16) {
+                const bool two = col0 + c + 8 < columns;
+                Added d0, d1;
+                read(d0, matrix + col0 + c, (int)row + r0);
+                if (two) read(d1, matrix + col0 + c + 8, (int)row + r0);
+                store_column(mine, r0, c, d0, matrix + col0 + c, (int)row + r0);
+                if (two) store_column(mine, r0, c + 8, d1, matrix + col0 + c + 8, (int)row + r0);
             }
         }
     }
+    __device__ __forceinline__ void store_row(const float *mine, int r, int i0, const Added &d, long long row, int col) const
+    {
+        const float4 s0 = tc::staged(mine, r, i0 / 4), s1 = tc::staged(mine, r, i0 / 4 + 1);
+        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        store(s, d, row, col, columns);
+    }
+    __device__ __forceinline__ void store_column(const float *mine, int r0, int c, const Added &d, long long row, int col) const
+    {
+        float s[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) s[j] = mine[32 * (r0 + j) + 4 * ((c / 4) ^ ((r0 + j) & 7)) + c % 4];
+        store(s, d, row, col, columns);
+    }
+    __device__ __forceinline__ void read(Added &d, long long row, int col) const
+    {
+        const long long at = row * stride + col;
+        if (d_hi) d.hi = *reinterpret_cast<const Pack<f16, 8> *>(d_hi + at);
+        if (d_lo) d.lo = *reinterpret_cast<const Pack<f16, 8> *>(d_lo + at);
+    }
     // columns [col, col + 8) of one row of the result; rows of the halves are padded to whole eights
-    __device__ __forceinline__ void store(const float (&s)[8], long long row, int col, int end) const
+    __device__ __forceinline__ void store(const float (&s)[8], const Added &d, long long row, int col, int end) const
     {
         float v[8];
         Pack<f16, 8> p, q;
         const long long at = row * stride + col;
-        if (d_hi) {
-            p = *reinterpret_cast<const Pack<f16, 8> *>(d_hi + at);
-            if (d_lo) q = *reinterpret_cast<const Pack<f16, 8> *>(d_lo + at);
-        }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             v[j] = beta * s[j];
-            if (d_hi) v[j] = fmaf(alpha, __half2float(p.v[j]) + (d_lo ? __half2float(q.v[j]) : 0.f), v[j]);
+            if (d_hi) v[j] = fmaf(alpha, __half2float(d.hi.v[j]) + (d_lo ? __half2float(d.lo.v[j]) : 0.f), v[j]);
         }
         if constexpr (FINAL) {
             T *to = result + row * columns + col;
@@ -339,6 +494,18 @@ extern "C" int ai2b_orthogonalize(int dtype, void *d_out, const void *d_g, int b
         const int s = m < n ? m : n, parts = (int)(size < NORM_BLOCKS * 1024LL ? (size + 1023) / 1024 : NORM_BLOCKS);
         double *norm = (double *)(ws + p.norm);
         const bool tensor = on_tensor_cores(m, n) && steps > 0;
+        if (!tensor && small_bytes(s, m < n ? n : m) <= SMALL_BYTES) {
+            const size_t smem = small_bytes(s, m < n ? n : m);
+            auto go = [&](auto kern, KernelSetup &ks) {
+                const int rc = kernel_setup(ks, kern, smem);
+                if (rc != AI2B_OK) return rc;
+                AI2B_CUDA(launch_chained(kern, dim3(batch), dim3(SMALL_THREADS), smem, st, (T *)d_out, (const T *)d_g, m, n, steps, (float)a, (float)b, (float)c, eps));
+                return (int)AI2B_OK;
+            };
+            // one result a thread while there are threads for all of the Gram matrix
+            static KernelSetup ks[2];
+            return s * s <= SMALL_THREADS ? go(small_kernel<T, 1>, ks[0]) : go(small_kernel<T, 4>, ks[1]);
+        }
         float *x = (float *)(ws + p.x[0]), *next = (float *)(ws + p.x[1]), *gram = (float *)(ws + p.gram), *poly = (float *)(ws + p.poly);
         AI2B_CUDA(launch_chained(norm_kernel<T>, dim3(parts, batch), dim3(256), 0, st, (const T *)d_g, size, norm));
         const int blocks = (int)(size < 512 * 256LL ? (size + 255) / 256 : 512);

@@ -167,7 +167,9 @@ __global__ void __launch_bounds__(256) dispatch_kernel(V *__restrict__ out, cons
     }
 }
 
-template <typename T, int N>
+// TOKENS accesses of different tokens and SLOTS of a token's slots are in flight at once: four in all, so that the rows of a token with one
+// slot do not wait for one another (1,048,576 x 64 floats: 145 us with one, 84 with four).
+template <typename T, int N, int TOKENS, int SLOTS>
 __global__ void __launch_bounds__(256) combine_kernel(Pack<T, N> *__restrict__ y, const Pack<T, N> *__restrict__ ys, long long ys_stride, const float *__restrict__ weights,
                                const int *__restrict__ position, long long tokens, int k, int per_row, long long rows)
 {
@@ -175,37 +177,43 @@ __global__ void __launch_bounds__(256) combine_kernel(Pack<T, N> *__restrict__ y
     chain_release();
     const long long total = tokens * per_row, step = (long long)gridDim.x * blockDim.x;
     const bool narrow = total <= 0xffffffffLL;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-        const long long t = row_of(i, per_row, narrow);
-        const int c = (int)(i - t * per_row);
-        float sum[N] = {};
-        for (int j0 = 0; j0 < k; j0 += 4) {      // four rows in flight
-            Pack<T, N> v[4];
-            float w[4];
+    for (long long i0 = (long long)blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += TOKENS * step) {
+        float sum[TOKENS][N] = {};
+        for (int j0 = 0; j0 < k; j0 += SLOTS) {
+            Pack<T, N> v[TOKENS][SLOTS];
+            float w[TOKENS][SLOTS];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                w[u] = 0.f;
-                if (j0 + u < k) {
-                    const int p = position[t * k + j0 + u];
-                    if (p >= 0 && p < rows) {
-                        w[u] = weights ? weights[t * k + j0 + u] : 1.f;
-                        v[u] = ys[p * ys_stride + c];
-                    } else {
-                        v[u] = Pack<T, N>{};     // a dropped slot adds zero whatever its weight and rows hold
+            for (int a = 0; a < TOKENS; a++) {
+                const long long i = min(i0 + a * step, total - 1), t = row_of(i, per_row, narrow);
+                const int c = (int)(i - t * per_row);
+#pragma unroll
+                for (int u = 0; u < SLOTS; u++) {
+                    w[a][u] = 0.f;
+                    v[a][u] = Pack<T, N>{};      // a dropped slot adds zero whatever its weight and rows hold
+                    if (j0 + u < k) {
+                        const int p = position[t * k + j0 + u];
+                        if (p >= 0 && p < rows) {
+                            w[a][u] = weights ? weights[t * k + j0 + u] : 1.f;
+                            v[a][u] = ys[p * ys_stride + c];
+                        }
                     }
-                } else {
-                    v[u] = Pack<T, N>{};
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 4; u++)
+            for (int a = 0; a < TOKENS; a++)
 #pragma unroll
-                for (int n = 0; n < N; n++) sum[n] = fmaf(w[u], to_float(v[u].v[n]), sum[n]);
+                for (int u = 0; u < SLOTS; u++)
+#pragma unroll
+                    for (int n = 0; n < N; n++) sum[a][n] = fmaf(w[a][u], to_float(v[a][u].v[n]), sum[a][n]);
         }
-        Pack<T, N> out;
 #pragma unroll
-        for (int n = 0; n < N; n++) out.v[n] = from_float<T>(sum[n]);
-        y[i] = out;
+        for (int a = 0; a < TOKENS; a++) {
+            if (i0 + a * step >= total) break;
+            Pack<T, N> out;
+#pragma unroll
+            for (int n = 0; n < N; n++) out.v[n] = from_float<T>(sum[a][n]);
+            y[i0 + a * step] = out;
+        }
     }
 }
 
@@ -338,7 +346,8 @@ using namespace ai2b;
 extern "C" size_t ai2b_route_workspace_bytes(long long tokens, int k, int experts)
 {
     if (tokens < 0 || k < 1 || experts < 1 || experts > MAX_EXPERTS) return 0;
-    return sizeof(int) * (size_t)plan_blocks(tokens * k, experts) * (experts + 1);
+    const int blocks = plan_blocks(tokens * k, experts);
+    return blocks > 1 ? sizeof(int) * (size_t)blocks * (experts + 1) : 0;
 }
 
 extern "C" int ai2b_route(const void *d_index, int index_is_i64, long long tokens, int k, int experts, int *d_order, int *d_position, int *d_offsets,
@@ -350,8 +359,9 @@ extern "C" int ai2b_route(const void *d_index, int index_is_i64, long long token
     AI2B_REQUIRE(experts <= MAX_EXPERTS, AI2B_ERR_UNSUPPORTED, "ai2b_route: at most %d experts (got %d)", MAX_EXPERTS, experts);
     const long long nslots = tokens * k;
     AI2B_REQUIRE(d_offsets && (nslots == 0 || (d_index && d_order && d_position)), AI2B_ERR_INVALID, "ai2b_route: NULL pointer");
-    AI2B_REQUIRE(d_workspace && workspace_bytes >= ai2b_route_workspace_bytes(tokens, k, experts), AI2B_ERR_WORKSPACE, "ai2b_route: workspace of %zu bytes, %zu needed",
-                 workspace_bytes, ai2b_route_workspace_bytes(tokens, k, experts));
+    const size_t need = ai2b_route_workspace_bytes(tokens, k, experts);
+    AI2B_REQUIRE(need == 0 || (d_workspace && workspace_bytes >= need), AI2B_ERR_WORKSPACE, "ai2b_route: workspace of %zu bytes, %zu needed",
+                 workspace_bytes, need);
     cudaStream_t st = (cudaStream_t)stream;
     return index_is_i64 ? route_plan((const long long *)d_index, nslots, experts, d_order, d_position, d_offsets, (int *)d_workspace, st)
                         : route_plan((const int *)d_index, nslots, experts, d_order, d_position, d_offsets, (int *)d_workspace, st);
@@ -384,13 +394,19 @@ extern "C" int ai2b_route_combine(int dtype, void *d_y, const void *d_ys, long l
     return with_pack(dtype, common_alignment(d_y, d_ys, size * width, size * ys_stride), [&](auto t, auto n) {
         using T = decltype(t);
         constexpr int N = decltype(n)::value;
-        static KernelSetup ks;
-        int grid;
-        const int rc2 = grid_for(ks, combine_kernel<T, N>, tokens * (width / N), &grid);
-        if (rc2 != AI2B_OK) return rc2;
-        AI2B_CUDA(launch_chained(combine_kernel<T, N>, dim3(grid), dim3(256), 0, (cudaStream_t)stream, (Pack<T, N> *)d_y, (const Pack<T, N> *)d_ys, ys_stride / N, d_weights,
-                                 d_position, tokens, k, width / N, tokens * k));
-        return (int)AI2B_OK;
+        const long long total = tokens * (width / N);
+        auto go = [&](auto kern, KernelSetup &ks, long long threads) {
+            int grid;
+            const int rc2 = grid_for(ks, kern, threads, &grid);
+            if (rc2 != AI2B_OK) return rc2;
+            AI2B_CUDA(launch_chained(kern, dim3(grid), dim3(256), 0, (cudaStream_t)stream, (Pack<T, N> *)d_y, (const Pack<T, N> *)d_ys, ys_stride / N, d_weights, d_position,
+                                     tokens, k, width / N, tokens * k));
+            return (int)AI2B_OK;
+        };
+        static KernelSetup ks[3];
+        if (k >= 3) return go(combine_kernel<T, N, 1, 4>, ks[0], total);
+        if (k == 2) return go(combine_kernel<T, N, 2, 2>, ks[1], (total + 1) / 2);
+        return go(combine_kernel<T, N, 4, 1>, ks[2], (total + 3) / 4);
     });
 }
 

@@ -66,9 +66,10 @@ variable_list route(const at::Tensor &index, int64_t experts)
     const auto opt = idx.options().dtype(at::kInt);
     at::Tensor order = at::empty({tokens * k}, opt), position = at::empty({tokens, k}, opt), offsets = at::empty({experts + 1}, opt);
     const size_t bytes = ai2b_route_workspace_bytes(tokens, (int)k, (int)experts);
-    at::Tensor ws = workspace(bytes, idx);
+    at::Tensor ws;
+    if (bytes > 0) ws = workspace(bytes, idx);
     check(ai2b_route(idx.data_ptr(), idx.scalar_type() == at::kLong, tokens, (int)k, (int)experts, order.data_ptr<int>(), position.data_ptr<int>(), offsets.data_ptr<int>(),
-                     ws.data_ptr(), bytes, stream()),
+                     ws.defined() ? ws.data_ptr() : nullptr, bytes, stream()),
           "ai2b_route");
     return {order, position, offsets};
 }

@@ -33,7 +33,7 @@ def test_route_refusals():
     refused(call(10, 1, 1025), -2, b"at most 1024")
     refused(call(2 ** 30, 2, 3), -2, b"2^31 - 1 slots")
     refused(call(10, 1, 3, index=NULL), -1, b"NULL")
-    refused(call(10, 1, 3, ws=NULL), -4, b"workspace")
+    refused(call(100000, 1, 3, ws=NULL), -4, b"workspace")
     refused(lib.ai2b_route_dispatch(C.c_int(9), ONE, ONE, C.c_longlong(4), ONE, C.c_longlong(2), C.c_int(1), C.c_int(4), NULL), -1, b"element type 9")
     refused(lib.ai2b_route_dispatch(F32, ONE, ONE, C.c_longlong(3), ONE, C.c_longlong(2), C.c_int(1), C.c_int(4), NULL), -1, b"row stride 3")
     refused(lib.ai2b_route_combine(F32, NULL, ONE, C.c_longlong(4), NULL, ONE, C.c_longlong(2), C.c_int(1), C.c_int(4), NULL), -1, b"NULL")
