@@ -41,27 +41,6 @@ __device__ __forceinline__ Activated activate(float z)
 // The same for results that are rounded to 16 bits, two at a time: the epilogue of a 16-bit layer is bound by the instructions that it issues
 // (39 per element with one at a time and expf's handling of subnormal numbers: 10,000 cycles for a tile whose products take 4,000).
 // Errors stay below 2^-20 of 1 + |z|.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
-{
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<unsigned long long &>(d))
-        : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)), "l"(reinterpret_cast<const unsigned long long &>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 exp2_2(float2 a)
 {
     float2 d;
@@ -110,11 +89,6 @@ __device__ __forceinline__ Activated2 activate2(float2 z)
     }
     return a;
 }
-
-__device__ __forceinline__ float2 widen(bf16 a, bf16 b) { return make_float2(__bfloat162float(a), __bfloat162float(b)); }
-__device__ __forceinline__ float2 widen(f16 a, f16 b) { return __half22float2(__halves2half2(a, b)); }
-__device__ __forceinline__ void narrow(bf16 *to, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(to) = __float22bfloat162_rn(v); }
-__device__ __forceinline__ void narrow(f16 *to, float2 v) { *reinterpret_cast<__half2 *>(to) = __float22half2_rn(v); }
 
 // ---- tiles of rows --------------------------------------------------------------------------------------------------------
 
@@ -307,43 +281,53 @@ __device__ __forceinline__ void split(float v, bf16 (&out)[PLANES])
     }
 }
 
-// Operand of a tensor-core product from rows that it cannot read as they are: 16-bit rows with other alignment are copied, floats
-// are cut into PLANES planes. out[plane][row][stride], `count` rows of `columns` each.
+// Operands of tensor-core products from rows that they cannot read as they are: 16-bit rows with other alignment are copied, floats
+// are cut into PLANES planes. out[plane][row][stride], `count` rows of `columns` each; two such copies in a launch, the first by `blocks` blocks.
 // A thread takes eight columns of a row; N: how many of them one access reads.
+template <typename T>
+struct PackJob {
+    void *out;
+    const T *in;
+    long long stride, in_stride, count;
+    int columns, blocks;
+};
 template <typename T, int PLANES, int N>
-__global__ void __launch_bounds__(256) pack_kernel(void *__restrict__ out, long long stride, const T *__restrict__ in, long long in_stride, long long count, int columns)
+__global__ void __launch_bounds__(256) pack_kernel(PackJob<T> first, PackJob<T> second)
 {
     using P = std::conditional_t<PLANES == 1, T, bf16>;
     chain_wait();
     chain_release();
-    const int per_row = (int)(stride / 8);
-    const long long total = count * per_row;
+    const bool other = (int)blockIdx.x >= first.blocks;
+    const PackJob<T> j = other ? second : first;
+    const long long block = blockIdx.x - (other ? first.blocks : 0), blocks = j.blocks;
+    const int per_row = (int)(j.stride / 8);
+    const long long total = j.count * per_row;
     const bool narrow = total <= 0xffffffffLL;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    for (long long i = block * blockDim.x + threadIdx.x; i < total; i += blocks * blockDim.x) {
         const long long r = row_of(i, per_row, narrow);
         const int c = (int)(i - r * per_row) * 8;
         T v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j += N) {
+        for (int u = 0; u < 8; u += N) {
             Pack<T, N> p{};
-            if (c + j < columns) p = *reinterpret_cast<const Pack<T, N> *>(in + r * in_stride + c + j);
+            if (c + u < j.columns) p = *reinterpret_cast<const Pack<T, N> *>(j.in + r * j.in_stride + c + u);
 #pragma unroll
-            for (int n = 0; n < N; n++) v[j + n] = p.v[n];
+            for (int n = 0; n < N; n++) v[u + n] = p.v[n];
         }
         Pack<P, 8> pieces[PLANES];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int u = 0; u < 8; u++) {
             if constexpr (PLANES == 1) {
-                pieces[0].v[j] = v[j];
+                pieces[0].v[u] = v[u];
             } else {
                 bf16 piece[PLANES];
-                split(to_float(v[j]), piece);
+                split(to_float(v[u]), piece);
 #pragma unroll
-                for (int p = 0; p < PLANES; p++) pieces[p].v[j] = piece[p];
+                for (int p = 0; p < PLANES; p++) pieces[p].v[u] = piece[p];
             }
         }
 #pragma unroll
-        for (int p = 0; p < PLANES; p++) *reinterpret_cast<Pack<P, 8> *>(reinterpret_cast<P *>(out) + (p * count + r) * stride + c) = pieces[p];
+        for (int p = 0; p < PLANES; p++) *reinterpret_cast<Pack<P, 8> *>(reinterpret_cast<P *>(j.out) + (p * j.count + r) * j.stride + c) = pieces[p];
     }
 }
 
@@ -855,19 +839,22 @@ static BackwardPlan plan_backward(const ai2b_dense *d)
     return p;
 }
 
+// Both operands of a call that need it, in one launch
 template <typename T>
-static int pack(const PackedRows &p, unsigned char *ws, cudaStream_t st)
+static int pack(const PackedRows &a, const PackedRows &b, unsigned char *ws, cudaStream_t st)
 {
-    if (!p.copy) return AI2B_OK;
-    const long long blocks = (p.count * p.stride() / 8 + 255) / 256;
+    if (!a.copy && !b.copy) return AI2B_OK;
     constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1, N = std::is_same<T, float>::value ? 4 : 1;
-    // (16-bit rows are copied because they are not aligned, float ones because they are float)
-    const bool vectors = N > 1 && common_alignment(p.from, 4 * p.from_stride, 4 * p.columns) >= 16;
-    auto go = [&](auto kern) {
-        return launch_chained(kern, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st, (void *)(ws + p.at), p.stride(), (const T *)p.from, p.from_stride,
-                              p.count, (int)p.columns);
+    auto job = [&](const PackedRows &p) {
+        const long long blocks = p.copy ? (p.count * p.stride() / 8 + 255) / 256 : 0;
+        return PackJob<T>{ws + p.at, (const T *)p.from, p.stride(), p.from_stride, p.count, (int)p.columns, (int)(blocks < 16384 ? blocks : 16384)};
     };
-    AI2B_CUDA(vectors ? go(pack_kernel<T, PLANES, N>) : go(pack_kernel<T, PLANES, 1>));
+    // (16-bit rows are copied because they are not aligned, float ones because they are float)
+    auto aligned = [](const PackedRows &p) { return !p.copy || common_alignment(p.from, 4 * p.from_stride, 4 * p.columns) >= 16; };
+    const PackJob<T> first = job(a), second = job(b);
+    const dim3 grid(first.blocks + second.blocks);
+    if (N > 1 && aligned(a) && aligned(b)) AI2B_CUDA(launch_chained(pack_kernel<T, PLANES, N>, grid, dim3(256), 0, st, first, second));
+    else AI2B_CUDA(launch_chained(pack_kernel<T, PLANES, 1>, grid, dim3(256), 0, st, first, second));
     return AI2B_OK;
 }
 
@@ -996,8 +983,7 @@ extern "C" int ai2b_dense_forward(const ai2b_dense *d, void *stream)
         const RowOutput<T> o{(T *)d->d_y, d->activation != AI2B_ACT_NONE ? (Slope<T> *)d->d_slope : nullptr, (const T *)d->d_bias, (const T *)d->d_residual, d->residual_stride,
                              d->activation};
         if (p.tensor) {
-            int rc2 = pack<T>(p.x, ws, st);
-            if (rc2 == AI2B_OK) rc2 = pack<T>(p.weight, ws, st);
+            int rc2 = pack<T>(p.x, p.weight, ws, st);
             if (rc2 == AI2B_OK) rc2 = multiply_rows<T, false>(d, p.x, p.weight, ws, o, d->inner, d->outer, st);
             return rc2;
         }
@@ -1039,12 +1025,18 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
                 if (p.tensor) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<T, T, 1, N>) : go(slope_kernel<T, T, 1, 1>));
             if (!p.tensor) AI2B_CUDA(p.vectors > 1 ? go(slope_kernel<T, float, 1, N>) : go(slope_kernel<T, float, 1, 1>));
         }
+        if (p.tensor) {
+            PackedRows w = p.weight, x = p.x;
+            w.copy = w.copy && d->d_gx;
+            x.copy = x.copy && d->d_gweight;
+            const int rc2 = pack<T>(w, x, ws, st);
+            if (rc2 != AI2B_OK) return rc2;
+        }
         const void *gz = p.gz.copy ? ws + p.gz.at : d->d_gy;      // (on the FMA pipes: float if made here, else gy)
         if (d->d_gx && d->rows > 0) {
             const RowOutput<T> o{(T *)d->d_gx, nullptr, nullptr, nullptr, 0, AI2B_ACT_NONE};
             if (p.tensor) {
-                int rc2 = pack<T>(p.weight, ws, st);
-                if (rc2 == AI2B_OK) rc2 = multiply_rows<T, true>(d, p.gz, p.weight, ws, o, d->outer, d->inner, st);
+                const int rc2 = multiply_rows<T, true>(d, p.gz, p.weight, ws, o, d->outer, d->inner, st);
                 if (rc2 != AI2B_OK) return rc2;
             } else {
                 const dim3 grid((unsigned)((d->rows + FT - 1) / FT + d->groups), (d->inner + FT - 1) / FT);
@@ -1057,8 +1049,7 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
         }
         if (d->d_gweight) {
             if (p.tensor) {
-                int rc2 = pack<T>(p.x, ws, st);
-                if (rc2 == AI2B_OK) rc2 = multiply_weight<T>(d, p, ws, wpart, st);
+                const int rc2 = multiply_weight<T>(d, p, ws, wpart, st);
                 if (rc2 != AI2B_OK) return rc2;
             } else if (d->rows > 0) {
                 const dim3 grid((unsigned)slab_bound(d->rows, p.weight_height, d->groups), (d->outer + FT - 1) / FT, (d->inner + FT - 1) / FT);

@@ -18,6 +18,33 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ bf16 from_float<bf16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ f16 from_float<f16>(float v) { return __float2half_rn(v); }
 
+// Two numbers at a time: one instruction for both, and one rounding of both
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)), "l"(reinterpret_cast<const unsigned long long &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 widen(bf16 a, bf16 b) { return make_float2(__bfloat162float(a), __bfloat162float(b)); }
+__device__ __forceinline__ float2 widen(f16 a, f16 b) { return __half22float2(__halves2half2(a, b)); }
+__device__ __forceinline__ void narrow(bf16 *to, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(to) = __float22bfloat162_rn(v); }
+__device__ __forceinline__ void narrow(f16 *to, float2 v) { *reinterpret_cast<__half2 *>(to) = __float22half2_rn(v); }
+
 // N consecutive elements that are loaded and stored at once (the address is a multiple of their size)
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Pack {

@@ -16,7 +16,8 @@
 
 namespace ai2b {
 
-constexpr int NORM_BLOCKS = 64;           // partial sums of squares per matrix
+// Partial sums of squares of a matrix: from its size alone, so that a matrix has the same norm whatever it is batched with
+static int norm_parts(long long size) { return (int)(size < 512 * 4096LL ? (size + 4095) / 4096 : 512); }
 
 // Squares are added in double: G may hold any float
 template <typename T>
@@ -36,17 +37,23 @@ __global__ void __launch_bounds__(256) norm_kernel(const T *__restrict__ g, long
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 8; w++) sum += sums[w];
-        part[blockIdx.y * NORM_BLOCKS + blockIdx.x] = sum;
+        part[blockIdx.y * gridDim.x + blockIdx.x] = sum;
     }
 }
 
-// 1 / (norm + eps) from the partial sums, the same in every thread of every block
+// 1 / (norm + eps) from the partial sums, the same in every thread of every block (the root and the quotient in double are one warp's work: in every
+// thread they took longer than the matrix)
 __device__ __forceinline__ double norm_scale(const double *part, int parts, double eps)
 {
-    const int lane = threadIdx.x & 31;
-    double sum = 0.0;
-    for (int i = lane; i < parts; i += 32) sum += part[i];
-    return 1.0 / (sqrt(warp_sum(sum)) + eps);
+    __shared__ double scale;
+    if (threadIdx.x < 32) {
+        double sum = 0.0;
+        for (int i = threadIdx.x; i < parts; i += 32) sum += part[i];
+        sum = warp_sum(sum);
+        if (threadIdx.x == 0) scale = 1.0 / (sqrt(sum) + eps);
+    }
+    __syncthreads();
+    return scale;
 }
 
 template <typename T>
@@ -54,7 +61,7 @@ __global__ void __launch_bounds__(256) normalise_kernel(float *__restrict__ x, c
 {
     chain_wait();
     chain_release();
-    const double scale = norm_scale(part + blockIdx.y * NORM_BLOCKS, parts, eps);
+    const double scale = norm_scale(part + blockIdx.y * (long long)parts, parts, eps);
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (long long)gridDim.x * blockDim.x)
         x[blockIdx.y * size + i] = (float)((double)to_float(g[blockIdx.y * size + i]) * scale);
 }
@@ -235,7 +242,7 @@ __global__ void __launch_bounds__(256) normalise_halves_kernel(f16 *__restrict__
 {
     chain_wait();
     chain_release();
-    const double scale = norm_scale(part + blockIdx.y * NORM_BLOCKS, parts, eps);
+    const double scale = norm_scale(part + blockIdx.y * (long long)parts, parts, eps);
     const long long size = (long long)m * n;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (long long)gridDim.x * blockDim.x) {
         const long long r = row_of(i, n, size <= 0xffffffffLL), at = (blockIdx.y * (long long)m + r) * stride + (i - r * n);
@@ -295,47 +302,39 @@ struct BatchOut {
     __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
     __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &) const
     {
-        const int i0 = lane % 4 * 8, col = col0 + i0;
+        // Pieces of eight columns of the results' rows; then, where the result is its own transpose, the same with rows and columns exchanged. The loops are not
+        // unrolled: a launch runs this code once or twice, and fetching it takes longer than running it.
         const long long matrix = (long long)it.batch * rows;
-        // (two rows at a time on their way: more do not fit the registers)
-        if (col < columns) {
+        const int across = lane % 4 * 8, down = lane / 4;
+        if (col0 + across < columns) {
+            const int last = (int)min((long long)32, it.row_end - row), col = col0 + across;
+            Added next, d;
+            if (down < last) read(next, matrix + row + down, col);
 #pragma unroll 1
-            for (int r = lane / 4; row + r < it.row_end && r < 32; r += 16) {
-                const bool two = row + r + 8 < it.row_end;
-                Added d0, d1;
-                read(d0, matrix + row + r, col);
-                if (two) read(d1, matrix + row + r + 8, col);
-                store_row(mine, r, i0, d0, matrix + row + r, col);
-                if (two) store_row(mine, r + 8, i0, d1, matrix + row + r + 8, col);
+            for (int r = down; r < last; r += 8) {
+                d = next;
+                if (r + 8 < last) read(next, matrix + row + r + 8, col);
+                const float4 s0 = tc::staged(mine, r, across / 4), s1 = tc::staged(mine, r, across / 4 + 1);
+                const float2 s[4] = {make_float2(s0.x, s0.y), make_float2(s0.z, s0.w), make_float2(s1.x, s1.y), make_float2(s1.z, s1.w)};
+                store(s, d, matrix + row + r, col, columns);
             }
         }
-        if (it.col >= it.mirror_from) {
-            // rows and columns exchanged: eight rows of the sums make up a piece of a row
-            const int r0 = lane % 4 * 8;
-            if (row + r0 >= it.row_end) return;
+        if (it.col >= it.mirror_from && row + across < it.row_end) {
+            const int last = min(32, columns - col0), col = (int)row + across;
+            Added next, d;
+            if (down < last) read(next, matrix + col0 + down, col);
 #pragma unroll 1
-            for (int c = lane / 4; col0 + c < columns && c < 32; c += 16) {
-                const bool two = col0 + c + 8 < columns;
-                Added d0, d1;
-                read(d0, matrix + col0 + c, (int)row + r0);
-                if (two) read(d1, matrix + col0 + c + 8, (int)row + r0);
-                store_column(mine, r0, c, d0, matrix + col0 + c, (int)row + r0);
-                if (two) store_column(mine, r0, c + 8, d1, matrix + col0 + c + 8, (int)row + r0);
-            }
-        }
-    }
-    __device__ __forceinline__ void store_row(const float *mine, int r, int i0, const Added &d, long long row, int col) const
-    {
-        const float4 s0 = tc::staged(mine, r, i0 / 4), s1 = tc::staged(mine, r, i0 / 4 + 1);
-        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-        store(s, d, row, col, columns);
-    }
-    __device__ __forceinline__ void store_column(const float *mine, int r0, int c, const Added &d, long long row, int col) const
-    {
-        float s[8];
+            for (int c = down; c < last; c += 8) {
+                d = next;
+                if (c + 8 < last) read(next, matrix + col0 + c + 8, col);
+                const float *from = mine + 32 * across + c % 4;
+                const int group = c / 4;
+                float2 s[4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) s[j] = mine[32 * (r0 + j) + 4 * ((c / 4) ^ ((r0 + j) & 7)) + c % 4];
-        store(s, d, row, col, columns);
+                for (int j = 0; j < 4; j++) s[j] = make_float2(from[64 * j + 4 * (group ^ (2 * j))], from[64 * j + 32 + 4 * (group ^ (2 * j + 1))]);
+                store(s, d, matrix + col0 + c, col, columns);
+            }
+        }
     }
     __device__ __forceinline__ void read(Added &d, long long row, int col) const
     {
@@ -344,29 +343,34 @@ struct BatchOut {
         if (d_lo) d.lo = *reinterpret_cast<const Pack<f16, 8> *>(d_lo + at);
     }
     // columns [col, col + 8) of one row of the result; rows of the halves are padded to whole eights
-    __device__ __forceinline__ void store(const float (&s)[8], const Added &d, long long row, int col, int end) const
+    __device__ __forceinline__ void store(const float2 (&s)[4], const Added &d, long long row, int col, int end) const
     {
-        float v[8];
-        Pack<f16, 8> p, q;
         const long long at = row * stride + col;
+        float2 v[4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            v[j] = beta * s[j];
-            if (d_hi) v[j] = fmaf(alpha, __half2float(d.hi.v[j]) + (d_lo ? __half2float(d.lo.v[j]) : 0.f), v[j]);
+        for (int j = 0; j < 4; j++) {
+            v[j] = mul2(s[j], both(beta));
+            if (d_hi) {
+                float2 a = widen(d.hi.v[2 * j], d.hi.v[2 * j + 1]);
+                if (d_lo) a = add2(a, widen(d.lo.v[2 * j], d.lo.v[2 * j + 1]));
+                v[j] = fma2(both(alpha), a, v[j]);
+            }
         }
         if constexpr (FINAL) {
             T *to = result + row * columns + col;
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (col + j < end) to[j] = from_float<T>(v[j] * (1.f / SCALE));
+                if (col + j < end) to[j] = from_float<T>((j & 1 ? v[j / 2].y : v[j / 2].x) * (1.f / SCALE));
         } else {
+            Pack<f16, 8> p;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                p.v[j] = __float2half_rn(v[j]);
-                q.v[j] = __float2half_rn(v[j] - __half2float(p.v[j]));
-            }
+            for (int j = 0; j < 4; j++) narrow(&p.v[2 * j], v[j]);
             *reinterpret_cast<Pack<f16, 8> *>(hi + at) = p;
-            if (lo) *reinterpret_cast<Pack<f16, 8> *>(lo + at) = q;
+            if (lo) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) narrow(&p.v[2 * j], fma2(widen(p.v[2 * j], p.v[2 * j + 1]), both(-1.f), v[j]));
+                *reinterpret_cast<Pack<f16, 8> *>(lo + at) = p;
+            }
         }
     }
 };
@@ -389,7 +393,7 @@ static OrthogonalizePlan plan_orthogonalize(int batch, int m, int n)
     const size_t xs = sizeof(float) * (size_t)batch * m * (tensor ? padded(n) : n), ss = sizeof(float) * (size_t)batch * s * (tensor ? padded(s) : s);
     size_t at = 0;
     p.norm = at;
-    at += round256(sizeof(double) * (size_t)batch * NORM_BLOCKS);
+    at += round256(sizeof(double) * (size_t)batch * norm_parts((long long)m * n));
     for (int i = 0; i < 2; i++) {
         p.x[i] = at;
         at += round256(xs);
@@ -491,7 +495,7 @@ extern "C" int ai2b_orthogonalize(int dtype, void *d_out, const void *d_g, int b
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         const long long size = (long long)m * n;
-        const int s = m < n ? m : n, parts = (int)(size < NORM_BLOCKS * 1024LL ? (size + 1023) / 1024 : NORM_BLOCKS);
+        const int s = m < n ? m : n, parts = norm_parts(size);
         double *norm = (double *)(ws + p.norm);
         const bool tensor = on_tensor_cores(m, n) && steps > 0;
         if (!tensor && small_bytes(s, m < n ? n : m) <= SMALL_BYTES) {
