@@ -587,19 +587,19 @@ struct RowOut {
     }
 
     template <int ACT, bool SLOPE>
-    __device__ __forceinline__ void apply(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &ahead) const
+    __device__ __forceinline__ void apply(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &ahead, bool dry) const
     {
-        const bool kept = it.batch < groups, add = o.residual && kept;
-        const int last = (int)min((long long)32, it.row_end - row);
+        const bool kept = it.batch < groups, add = o.residual && kept && !dry;
+        const int last = dry ? (vectors ? ROWS : 2) : (int)min((long long)32, it.row_end - row);
         if (!vectors) {
             // a column a lane, two rows at a time (eight columns a lane, element by element, took 6 us more for each 1157 x 97 results)
             const int col = col0 + lane;
             if (col >= columns) return;
-            const float bias = o.bias && kept ? to_float(o.bias[(long long)it.batch * columns + col]) : 0.f;
+            const float bias = o.bias && kept && !dry ? to_float(o.bias[(long long)it.batch * columns + col]) : 0.f;
 #pragma unroll 2
             for (int r = 0; r < last; r += 2) {
                 const long long at = row + r;
-                const bool two = r + 1 < last;
+                const bool two = r + 1 < last && !dry;
                 float2 z;
                 z.x = mine[32 * r + 4 * ((lane / 4) ^ (r & 7)) + lane % 4] + bias;
                 z.y = mine[32 * (r + 1) + 4 * ((lane / 4) ^ ((r + 1) & 7)) + lane % 4] + bias;
@@ -608,10 +608,10 @@ struct RowOut {
                     a.value.x += to_float(o.residual[at * o.residual_stride + col]);
                     if (two) a.value.y += to_float(o.residual[(at + 1) * o.residual_stride + col]);
                 }
-                o.out[at * columns + col] = from_float<T>(a.value.x);
+                if (!dry) o.out[at * columns + col] = from_float<T>(a.value.x);
                 if (two) o.out[(at + 1) * columns + col] = from_float<T>(a.value.y);
                 if constexpr (SLOPE) {
-                    o.slope[at * columns + col] = from_float<Slope<T>>(a.slope.x);
+                    if (!dry) o.slope[at * columns + col] = from_float<Slope<T>>(a.slope.x);
                     if (two) o.slope[(at + 1) * columns + col] = from_float<Slope<T>>(a.slope.y);
                 }
             }
@@ -654,26 +654,26 @@ struct RowOut {
                     slope.v[j + 1] = a.slope.y;
                 }
             }
-            *reinterpret_cast<Pack<T, N> *>(py) = y;
+            if (!dry) *reinterpret_cast<Pack<T, N> *>(py) = y;
             if constexpr (SLOPE) {
-                *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
+                if (!dry) *reinterpret_cast<Pack<Slope<T>, N> *>(ps) = slope;
                 ps += ROWS * (long long)columns;
             }
         }
     }
     template <int ACT>
-    __device__ __forceinline__ void choose(const tc::Item &it, long long row, int col, const float *mine, int lane, const Ahead &ahead) const
+    __device__ __forceinline__ void choose(const tc::Item &it, long long row, int col, const float *mine, int lane, const Ahead &ahead, bool dry) const
     {
-        if (ACT != AI2B_ACT_NONE && o.slope) apply<ACT, true>(it, row, col, mine, lane, ahead);
-        else apply<ACT, false>(it, row, col, mine, lane, ahead);
+        if (ACT != AI2B_ACT_NONE && o.slope) apply<ACT, true>(it, row, col, mine, lane, ahead, dry);
+        else apply<ACT, false>(it, row, col, mine, lane, ahead, dry);
     }
-    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col, const float *mine, int lane, const Ahead &ahead) const
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col, const float *mine, int lane, const Ahead &ahead, bool dry) const
     {
         switch (o.activation) {
-        case AI2B_ACT_TANH: choose<AI2B_ACT_TANH>(it, row, col, mine, lane, ahead); break;
-        case AI2B_ACT_SILU: choose<AI2B_ACT_SILU>(it, row, col, mine, lane, ahead); break;
-        case AI2B_ACT_GELU: choose<AI2B_ACT_GELU>(it, row, col, mine, lane, ahead); break;
-        default: choose<AI2B_ACT_NONE>(it, row, col, mine, lane, ahead);
+        case AI2B_ACT_TANH: choose<AI2B_ACT_TANH>(it, row, col, mine, lane, ahead, dry); break;
+        case AI2B_ACT_SILU: choose<AI2B_ACT_SILU>(it, row, col, mine, lane, ahead, dry); break;
+        case AI2B_ACT_GELU: choose<AI2B_ACT_GELU>(it, row, col, mine, lane, ahead, dry); break;
+        default: choose<AI2B_ACT_NONE>(it, row, col, mine, lane, ahead, dry);
         }
     }
 };
@@ -708,13 +708,13 @@ struct WeightOut {
     bool vectors;
     struct Ahead {};
     __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
-    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &) const
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &, bool dry) const
     {
         const int i = lane & 7, col = col0 + 4 * i;
         if (col >= columns) return;
 #pragma unroll
         for (int r = lane >> 3; r < 32; r += 4) {
-            if (row + r >= it.row_end) return;
+            if (row + r >= it.row_end || dry) return;
             const float4 v = tc::staged(mine, r, i);
             float *p = part + ((long long)it.batch * outer + row + r) * columns + col;
             if (vectors) {

@@ -204,7 +204,8 @@ struct Operands {
 
 // Items::prepare(table), by all threads, may leave something in shared memory; Items::get(table, t, item), by whole warps, gives tile t, false after
 // the last one. (table is NULL, and nothing was prepared, where there is no room for it.) Out takes 32 x 32 sums at a time, in shared memory:
-// out.load(ahead, item, first row, first column, lane) reads what it needs of memory, out(item, first row, first column, sums, lane, ahead) stores.
+// out.load(ahead, item, first row, first column, lane) reads what it needs of memory, out(item, first row, first column, sums, lane, ahead, dry) stores;
+// dry: one pass through its code, with no access to memory.
 template <int PLANES, int BN, bool PAIR, bool A_MN, bool B_MN, typename Items, typename Out>
 __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLANES, BN, PAIR>::THREADS, 1) product_kernel(const __grid_constant__ Operands ops, const __grid_constant__ Items items, const __grid_constant__ Out out)
 {
@@ -237,6 +238,11 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
         *stopped = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    if (warp == 2 && elect_one()) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&ops.a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&ops.b) : "memory");
+        if (ops.ahead_columns > 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&ops.ahead) : "memory");
     }
     if (warp == 1) {
         if constexpr (PAIR) {
@@ -384,15 +390,20 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
         unsigned sets = 0;
         // Lane l holds row l of 32 sums: through shared memory, so that neighbouring lanes get neighbouring columns. Four columns at a time, permuted
         // within the row, keep both directions free of bank conflicts.
-        auto hand_over = [&](const float (&v)[32], long long row, int col, const typename Out::Ahead &ahead) {
+        auto hand_over = [&](const float (&v)[32], long long row, int col, const typename Out::Ahead &ahead, bool dry) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 *reinterpret_cast<float4 *>(mine + 32 * lane + 4 * (i ^ (lane & 7))) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             __syncwarp();
-            out(it, row, col, mine, lane, ahead);
+            out(it, row, col, mine, lane, ahead, dry);
             __syncwarp();
         };
-        for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
+        // The first round is a dry one: one pass over sums of zero, nothing read of memory or stored. It brings the epilogue's code into the
+        // caches while the first products are under way; fetching it then, line after line, took 4,400 cycles of a tile of 128 x 128.
+        bool dry = true;
+        for (long long t = first_tile; ok;) {
+            if (dry) it = Item{0, 0, 0, 0, 0, 0, 0, 32 * (long long)(quarter + 1) + rank * BM, 0, 0, 0};
+            else if (!items.get(table, t, it)) break;
             const long long row = it.row + rank * BM + 32 * quarter;
             constexpr int PARTS = (BN + 32 * S::SHARES - 1) / (32 * S::SHARES);
             float sum[S::CAREFUL ? PARTS : 1][32];
@@ -401,11 +412,12 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                 for (int i = 0; i < PARTS; i++)
 #pragma unroll
                     for (int j = 0; j < 32; j++) sum[i][j] = 0.f;
-                for (int k0 = it.k_begin; k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end, sets++) {
-                    ok = barrier_wait(done + 8 * (sets & 1), (sets >> 1) & 1);
+                for (int k0 = it.k_begin; k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end) {
+                    const unsigned set = sets & 1;
+                    ok = barrier_wait(done + 8 * set, (sets >> 1) & 1);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned from = tmem + (sets & 1) * S::ACCUMULATORS * BN + 32 * share + ((unsigned)(32 * quarter) << 16);
+                    const unsigned from = tmem + set * S::ACCUMULATORS * BN + 32 * share + ((unsigned)(32 * quarter) << 16);
 #pragma unroll
                     for (int i = 0; i < PARTS; i++) {
                         if (32 * (share + S::SHARES * i) >= BN) break;
@@ -416,7 +428,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                         for (int j = 0; j < 32; j++) sum[i][j] += v[j] + low[j];
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    if (lane == 0) barrier_arrive(taken_of_pair + 8 * (sets & 1));
+                    if (lane == 0) barrier_arrive(taken_of_pair + 8 * set);
+                    sets++;
                 }
                 if (!ok) break;
 #pragma unroll
@@ -424,8 +437,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                     const int c = 32 * (share + S::SHARES * i);
                     if (c < BN && row < it.row_end && it.col + c < out.columns) {
                         typename Out::Ahead ahead;
-                        out.load(ahead, it, row, it.col + c, lane);
-                        hand_over(sum[i], row, it.col + c, ahead);
+                        if (!dry) out.load(ahead, it, row, it.col + c, lane);
+                        hand_over(sum[i], row, it.col + c, ahead, dry);
                     }
                 }
             } else {
@@ -434,7 +447,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                 // What the epilogue reads of memory is asked for before the sums are there. (For the columns after the first 32 there are no registers
                 // to do it while those are worked on.)
                 typename Out::Ahead ahead;
-                if (32 * share < BN && row < it.row_end && it.col + 32 * share < out.columns) out.load(ahead, it, row, it.col + 32 * share, lane);
+                if (!dry && 32 * share < BN && row < it.row_end && it.col + 32 * share < out.columns) out.load(ahead, it, row, it.col + 32 * share, lane);
                 if (sums) {
                     ok = barrier_wait(done + 8 * set, (sets >> 1) & 1);
                     if (!ok) break;
@@ -449,7 +462,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
 #pragma unroll
                         for (int j = 0; j < 32; j++) sum[0][j] = 0.f;
                     }
-                    hand_over(sum[0], row, it.col + c, ahead);
+                    hand_over(sum[0], row, it.col + c, ahead, dry);
+                    if (dry) break;
                 }
                 if (sums) {
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -457,6 +471,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
                     sets++;
                 }
             }
+            if (dry) dry = false;
+            else t += tile_step;
         }
     }
     if (!ok && lane == 0) {
@@ -554,7 +570,7 @@ inline double tile_cost(Tile t, int planes, long long rows, long long edges, lon
     const double waves = (double)(long long)((tiles + sms / (t.pair ? 2 : 1) - 1) / (sms / (t.pair ? 2 : 1)));
     const double stages = (double)((inner + BK - 1) / BK), epilogue = 22.0 * t.columns;
     const double tile = stages * (products > copies ? products : copies);
-    return waves * (tile > epilogue ? tile : epilogue) + epilogue + 1500.0;
+    return waves * (tile > epilogue ? tile : epilogue) + epilogue + (t.pair ? 3500.0 : 1500.0);      // (a pair waits for both blocks)
 }
 // The kind that takes least. (Planes need two accumulators for each of two tiles: 128 columns at most.)
 inline Tile best_tile(int planes, long long rows, long long edges, long long columns, long long matrices, long long inner, int sms)

@@ -295,34 +295,52 @@ struct BatchOut {
     long long stride;                     // of the halves' rows, a multiple of 8
     bool symmetric;                       // (host) the result is its own transpose
 
-    struct Ahead {};
+    bool vectors;                         // the result's rows start at multiples of eight elements, and end there
+
     struct Added {
         Pack<f16, 8> hi, lo;
     };
-    __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
-    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &) const
+    using Ahead = Added;                  // of the first pass
+    __device__ __forceinline__ void load(Ahead &a, const tc::Item &it, long long row, int col0, int lane) const
+    {
+        if (col0 + lane % 4 * 8 < columns && row + lane / 4 < it.row_end) read(a, (long long)it.batch * rows + row + lane / 4, col0 + lane % 4 * 8);
+    }
+    __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &ahead, bool dry) const
     {
         // Pieces of eight columns of the results' rows; then, where the result is its own transpose, the same with rows and columns exchanged. The loops are not
         // unrolled: a launch runs this code once or twice, and fetching it takes longer than running it.
         const long long matrix = (long long)it.batch * rows;
         const int across = lane % 4 * 8, down = lane / 4;
+        if (FINAL && !vectors) {
+            // a column a lane
+            const int col = col0 + lane, last = dry ? 1 : (int)min((long long)32, it.row_end - row);
+            if (col >= columns) return;
+#pragma unroll 2
+            for (int r = 0; r < last; r++) {
+                const long long at = (matrix + row + r) * stride + col;
+                float v = beta * mine[32 * r + 4 * ((lane / 4) ^ (r & 7)) + lane % 4];
+                if (dry) continue;
+                v = fmaf(alpha, __half2float(d_hi[at]) + __half2float(d_lo[at]), v);
+                result[(matrix + row + r) * columns + col] = from_float<T>(v * (1.f / SCALE));
+            }
+            return;
+        }
         if (col0 + across < columns) {
-            const int last = (int)min((long long)32, it.row_end - row), col = col0 + across;
-            Added next, d;
-            if (down < last) read(next, matrix + row + down, col);
+            const int last = dry ? 8 : (int)min((long long)32, it.row_end - row), col = col0 + across;
+            Added next = ahead, d;
 #pragma unroll 1
             for (int r = down; r < last; r += 8) {
                 d = next;
                 if (r + 8 < last) read(next, matrix + row + r + 8, col);
                 const float4 s0 = tc::staged(mine, r, across / 4), s1 = tc::staged(mine, r, across / 4 + 1);
                 const float2 s[4] = {make_float2(s0.x, s0.y), make_float2(s0.z, s0.w), make_float2(s1.x, s1.y), make_float2(s1.z, s1.w)};
-                store(s, d, matrix + row + r, col, columns);
+                store(s, d, matrix + row + r, col, dry);
             }
         }
         if (it.col >= it.mirror_from && row + across < it.row_end) {
-            const int last = min(32, columns - col0), col = (int)row + across;
+            const int last = dry ? 8 : min(32, columns - col0), col = (int)row + across;
             Added next, d;
-            if (down < last) read(next, matrix + col0 + down, col);
+            if (down < last && !dry) read(next, matrix + col0 + down, col);
 #pragma unroll 1
             for (int c = down; c < last; c += 8) {
                 d = next;
@@ -332,7 +350,7 @@ struct BatchOut {
                 float2 s[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) s[j] = make_float2(from[64 * j + 4 * (group ^ (2 * j))], from[64 * j + 32 + 4 * (group ^ (2 * j + 1))]);
-                store(s, d, matrix + col0 + c, col, columns);
+                store(s, d, matrix + col0 + c, col, dry);
             }
         }
     }
@@ -343,7 +361,7 @@ struct BatchOut {
         if (d_lo) d.lo = *reinterpret_cast<const Pack<f16, 8> *>(d_lo + at);
     }
     // columns [col, col + 8) of one row of the result; rows of the halves are padded to whole eights
-    __device__ __forceinline__ void store(const float2 (&s)[4], const Added &d, long long row, int col, int end) const
+    __device__ __forceinline__ void store(const float2 (&s)[4], const Added &d, long long row, int col, bool dry) const
     {
         const long long at = row * stride + col;
         float2 v[4];
@@ -357,19 +375,19 @@ struct BatchOut {
             }
         }
         if constexpr (FINAL) {
-            T *to = result + row * columns + col;
+            Pack<T, 8> p;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (col + j < end) to[j] = from_float<T>((j & 1 ? v[j / 2].y : v[j / 2].x) * (1.f / SCALE));
+            for (int j = 0; j < 8; j++) p.v[j] = from_float<T>((j & 1 ? v[j / 2].y : v[j / 2].x) * (1.f / SCALE));
+            if (!dry) *reinterpret_cast<Pack<T, 8> *>(result + row * columns + col) = p;
         } else {
             Pack<f16, 8> p;
 #pragma unroll
             for (int j = 0; j < 4; j++) narrow(&p.v[2 * j], v[j]);
-            *reinterpret_cast<Pack<f16, 8> *>(hi + at) = p;
+            if (!dry) *reinterpret_cast<Pack<f16, 8> *>(hi + at) = p;
             if (lo) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) narrow(&p.v[2 * j], fma2(widen(p.v[2 * j], p.v[2 * j + 1]), both(-1.f), v[j]));
-                *reinterpret_cast<Pack<f16, 8> *>(lo + at) = p;
+                if (!dry) *reinterpret_cast<Pack<f16, 8> *>(lo + at) = p;
             }
         }
     }
@@ -451,10 +469,10 @@ static int iterate_tc(T *result, Halves x, Halves next, const Halves &gram, cons
     constexpr bool TWO = PLANES == 2;
     constexpr float UNSCALE = 1.f / SCALE;      // a product of two scaled numbers has one scale too many
     for (int i = 0; i < steps; i++) {
-        const BatchOut<T, false> to_gram{0.f, UNSCALE, nullptr, nullptr, gram.hi, TWO ? gram.lo : nullptr, nullptr, s, s, gram.stride, true};
-        const BatchOut<T, false> to_poly{b, c * UNSCALE, gram.hi, TWO ? gram.lo : nullptr, poly.hi, TWO ? poly.lo : nullptr, nullptr, s, s, poly.stride, true};
-        const BatchOut<T, false> to_next{a, UNSCALE, x.hi, x.lo, next.hi, next.lo, nullptr, n, m, x.stride, false};
-        const BatchOut<T, true> to_result{a, UNSCALE, x.hi, x.lo, nullptr, nullptr, result, n, m, x.stride, false};
+        const BatchOut<T, false> to_gram{0.f, UNSCALE, nullptr, nullptr, gram.hi, TWO ? gram.lo : nullptr, nullptr, s, s, gram.stride, true, true};
+        const BatchOut<T, false> to_poly{b, c * UNSCALE, gram.hi, TWO ? gram.lo : nullptr, poly.hi, TWO ? poly.lo : nullptr, nullptr, s, s, poly.stride, true, true};
+        const BatchOut<T, false> to_next{a, UNSCALE, x.hi, x.lo, next.hi, next.lo, nullptr, n, m, x.stride, false, true};
+        const BatchOut<T, true> to_result{a, UNSCALE, x.hi, x.lo, nullptr, nullptr, result, n, m, x.stride, false, n % 8 == 0 && common_alignment(result) >= 16 && (sizeof(T) == 2 || ((size_t)result & 31) == 0)};
         int rc = product_tc<PLANES, !WIDE, !WIDE>(x, x, to_gram, l, batch, st);
         if (rc == AI2B_OK) rc = product_tc<PLANES, false, false>(gram, gram, to_poly, s, batch, st);
         if (rc == AI2B_OK) {
