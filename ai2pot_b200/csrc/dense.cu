@@ -417,23 +417,17 @@ struct SlabSum {
     int height, blocks;           // blocks of the grid's x that belong to it
 };
 template <typename T, int N>
-__global__ void __launch_bounds__(256) sum_slabs_kernel(SlabSum<T> a, SlabSum<T> b, const int *__restrict__ offsets, long long rows)
+__device__ __forceinline__ void sum_slabs(const SlabSum<T> &j, int block, int e, const int *offsets, long long rows, long long *shared)
 {
-    __shared__ long long first_slab;
-    chain_wait();
-    chain_release();
-    const bool second = (int)blockIdx.x >= a.blocks;
-    const SlabSum<T> &j = second ? b : a;
-    const int e = blockIdx.y, block = blockIdx.x - (second ? a.blocks : 0);
     if (threadIdx.x < 32) {
         const long long n = tiles_before(offsets, e, rows, j.height);
-        if (threadIdx.x == 0) first_slab = n;
+        if (threadIdx.x == 0) shared[0] = n;
     }
     __syncthreads();
     const RowRange r = group_rows(offsets, e, rows);
     // (`slabs` are there, whatever the offsets say)
-    const int n = (int)min(tiles_of(r.end - r.begin, j.height), j.slabs - first_slab);
-    const float *part = j.part + first_slab * j.size;
+    const int n = (int)min(tiles_of(r.end - r.begin, j.height), j.slabs - shared[0]);
+    const float *part = j.part + shared[0] * j.size;
     for (long long i = ((long long)block * blockDim.x + threadIdx.x) * N; i < j.size; i += (long long)j.blocks * blockDim.x * N) {
         float sum[N] = {};
 #pragma unroll 4
@@ -447,6 +441,15 @@ __global__ void __launch_bounds__(256) sum_slabs_kernel(SlabSum<T> a, SlabSum<T>
         for (int c = 0; c < N; c++) out.v[c] = from_float<T>(sum[c]);
         *reinterpret_cast<Pack<T, N> *>(j.out + e * j.size + i) = out;
     }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) sum_slabs_kernel(SlabSum<T> a, SlabSum<T> b, const int *__restrict__ offsets, long long rows)
+{
+    __shared__ long long shared[1];
+    chain_wait();
+    chain_release();
+    if ((int)blockIdx.x < a.blocks) sum_slabs<T, 1>(a, blockIdx.x, blockIdx.y, offsets, rows, shared);
+    else sum_slabs<T, 1>(b, blockIdx.x - a.blocks, blockIdx.y, offsets, rows, shared);
 }
 
 // ---- products on the tensor cores -------------------------------------------------------------------------------------------
@@ -678,56 +681,177 @@ struct RowOut {
     }
 };
 
-// Tiles of gz^T x over the rows of one slab
+// gz^T x. The stages (64 rows) of all groups are one line, cut into `slabs` equal pieces; a block (pair) takes a tile of the result through a
+// slab, and stores a partial sum for each group that it meets there: slot (group + slab, tile). Those of a group are added in the order of the slabs.
+// Equal slabs keep the blocks busy whatever the groups' sizes are, and the blocks of a slab read the same rows at the same time. (65536 x 1024 x 1024 in
+// eight uneven groups: 125 to 148 us with slabs that end at groups; 142 us where the tiles, too, were on the line, because rows then come from memory
+// for each tile.)
+struct WeightLine {
+    const int *offsets;
+    int groups, tiles, slabs, units;      // tiles of a group's result; blocks (pairs)
+    long long rows;
+    static constexpr int LEAST = 4;       // stages of a slab
+
+    // Whole warps. Stages before group e, and of all groups
+    __device__ __forceinline__ void measure(int e, long long &before, long long &total) const
+    {
+        long long b = 0, n = 0;
+        for (int i = threadIdx.x & 31; i < groups; i += 32) {
+            const RowRange r = group_rows(offsets, i, rows);
+            const long long stages = tiles_of(r.end - r.begin, tc::BK);
+            n += stages;
+            if (i < e) b += stages;
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+            b += __shfl_xor_sync(FULL_MASK, b, o);
+            n += __shfl_xor_sync(FULL_MASK, n, o);
+        }
+        before = b;
+        total = n;
+    }
+    __device__ __forceinline__ long long piece(long long total) const { return max((total + slabs - 1) / slabs, (long long)LEAST); }
+    // Whole warps: group of the stage at `at`, and the stages before that group; -1 behind the end
+    __device__ __forceinline__ int group_at(long long at, long long &before) const
+    {
+        const int lane = threadIdx.x & 31;
+        long long base = 0;
+        for (int e0 = 0; e0 < groups; e0 += 32) {
+            long long mine = 0;
+            if (e0 + lane < groups) {
+                const RowRange r = group_rows(offsets, e0 + lane, rows);
+                mine = tiles_of(r.end - r.begin, tc::BK);
+            }
+            long long scan = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long up = __shfl_up_sync(FULL_MASK, scan, o);
+                if (lane >= o) scan += up;
+            }
+            const unsigned hit = __ballot_sync(FULL_MASK, base + scan > at);
+            if (hit) {
+                before = base + __shfl_sync(FULL_MASK, scan - mine, __ffs(hit) - 1);
+                return e0 + __ffs(hit) - 1;
+            }
+            base += __shfl_sync(FULL_MASK, scan, 31);
+        }
+        return -1;
+    }
+};
 template <int BN>
 struct WeightItems {
-    GroupTable of;
-    int tile_rows, row_tiles, column_tiles, outer;
-    __device__ __forceinline__ void prepare(int *table) const { of.prepare(table); }
-    __device__ __forceinline__ bool get(const int *table, long long t, tc::Item &it) const
+    WeightLine line;
+    int tile_rows, column_tiles, outer;
+    __device__ __forceinline__ void prepare(int *) const {}
+    __device__ __forceinline__ bool get(const int *, long long t, tc::Item &it) const
     {
-        const int per_slab = row_tiles * column_tiles;
-        const long long slab = row_of(t, per_slab, t <= 0xffffffffLL);
-        const RowTile tile = of.find(table, slab);
-        if (tile.group < 0 || tile.group >= of.groups) return false;
-        const int i = (int)(t - slab * per_slab);
-        it.a_at = i / column_tiles * tile_rows;
-        it.b_at = it.col = i % column_tiles * BN;
+        // t: the block's own index at first; later ones are kept here, because a slab may give several tiles
+        long long before, total;
+        line.measure(0, before, total);
+        const long long piece = line.piece(total);
+        if (it.cursor < 0) {
+            it.mirror_from = (int)t;
+            it.cursor = t / line.tiles * piece;
+        }
+        long long end;
+        while (end = min((it.mirror_from / line.tiles + 1) * piece, total), it.cursor >= end) {
+            it.mirror_from += line.units;
+            if (it.mirror_from >= line.slabs * line.tiles) return false;
+            it.cursor = it.mirror_from / line.tiles * piece;
+        }
+        const int e = line.group_at(it.cursor, before);
+        if (e < 0) return false;
+        const RowRange r = group_rows(line.offsets, e, line.rows);
+        const long long first = it.cursor - before, last = min(tiles_of(r.end - r.begin, tc::BK), first + end - it.cursor);
+        const int tile = it.mirror_from % line.tiles;
+        it.a_at = tile / column_tiles * tile_rows;
+        it.b_at = it.col = tile % column_tiles * BN;
         it.a_batch = it.b_batch = 0;
-        it.k_begin = (int)tile.begin;
-        it.k_end = (int)tile.end;
+        it.k_begin = (int)(r.begin + first * tc::BK);
+        it.k_end = (int)min(r.begin + last * tc::BK, r.end);
         it.row = it.a_at;
         it.row_end = outer;
-        it.batch = (int)slab;
+        it.batch = (e + it.mirror_from / line.tiles) * line.tiles + tile;
+        it.cursor += last - first;
         return true;
     }
 };
 struct WeightOut {
-    float *part;              // [slab][outer][inner]
-    int columns, outer;
-    bool vectors;
+    float *part;              // [slot][tile_rows][tile_columns]
+    int columns, tile_rows, tile_columns;
+    static constexpr bool BY_ROWS = false;
     struct Ahead {};
     __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
     __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &, bool dry) const
     {
-        const int i = lane & 7, col = col0 + 4 * i;
-        if (col >= columns) return;
+        const int i = lane & 7;
+        float *to = part + ((long long)it.batch * tile_rows + (row - it.row)) * tile_columns + (col0 - it.col) + 4 * i;
 #pragma unroll
-        for (int r = lane >> 3; r < 32; r += 4) {
-            if (row + r >= it.row_end || dry) return;
-            const float4 v = tc::staged(mine, r, i);
-            float *p = part + ((long long)it.batch * outer + row + r) * columns + col;
-            if (vectors) {
-                *reinterpret_cast<float4 *>(p) = v;
-            } else {
-                p[0] = v.x;
-                if (col + 1 < columns) p[1] = v.y;
-                if (col + 2 < columns) p[2] = v.z;
-                if (col + 3 < columns) p[3] = v.w;
-            }
-        }
+        for (int r = lane >> 3; r < 32; r += 4)
+            if (!dry) *reinterpret_cast<float4 *>(to + r * tile_columns) = tc::staged(mine, r, i);
     }
 };
+
+// The weight gradient from its partial sums, a row of a tile at a time, and the bias gradient from those of slope_kernel
+template <typename T>
+struct PieceSum {
+    T *out;
+    const float *part;
+    WeightLine line;
+    int tile_rows, tile_columns, column_tiles, outer, inner, blocks;      // blocks per group
+    bool vectors;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) sum_pieces_kernel(PieceSum<T> w, SlabSum<T> b, const int *__restrict__ offsets, long long rows)
+{
+    __shared__ long long shared[2];
+    chain_wait();
+    chain_release();
+    if ((int)blockIdx.x >= w.blocks) {
+        sum_slabs<T, 1>(b, blockIdx.x - w.blocks, blockIdx.y, offsets, rows, shared);
+        return;
+    }
+    const int e = blockIdx.y;
+    if (threadIdx.x < 32) {
+        long long before, total;
+        w.line.measure(e, before, total);
+        if (threadIdx.x == 0) {
+            shared[0] = before;
+            shared[1] = w.line.piece(total);
+        }
+    }
+    __syncthreads();
+    const RowRange r = group_rows(offsets, e, rows);
+    const long long stages = tiles_of(r.end - r.begin, tc::BK), size = (long long)w.tile_rows * w.tile_columns, fours = size / 4;
+    T *out = w.out + (long long)e * w.outer * w.inner;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < fours * w.line.tiles; i += (long long)w.blocks * blockDim.x) {
+        const int tile = (int)(i / fours), at = (int)(i - tile * fours) * 4;
+        const int row = tile / w.column_tiles * w.tile_rows + at / w.tile_columns, col = tile % w.column_tiles * w.tile_columns + at % w.tile_columns;
+        if (row >= w.outer || col >= w.inner) continue;
+        float sum[4] = {};
+        if (stages > 0) {
+            const long long s1 = (shared[0] + stages - 1) / shared[1];
+            for (long long s = shared[0] / shared[1]; s <= s1; s++) {
+                const float4 v = *reinterpret_cast<const float4 *>(w.part + ((e + s) * w.line.tiles + tile) * size + at);
+                sum[0] += v.x;
+                sum[1] += v.y;
+                sum[2] += v.z;
+                sum[3] += v.w;
+            }
+        }
+        T *to = out + (long long)row * w.inner + col;
+        if (w.vectors) {
+            Pack<T, 4> p;
+#pragma unroll
+            for (int j = 0; j < 4; j++) p.v[j] = from_float<T>(sum[j]);
+            *reinterpret_cast<Pack<T, 4> *>(to) = p;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (col + j < w.inner) to[j] = from_float<T>(sum[j]);
+        }
+    }
+}
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 
@@ -792,10 +916,41 @@ static ForwardPlan plan_forward(const ai2b_dense *d)
     return p;
 }
 
+// The tile of the weight gradient's products and the number of slabs that take least, in cycles: rounds of blocks, each as long as the stages of a slab and
+// an epilogue (22 cycles a column), and 8 bytes of every partial sum, written and read at 3400 bytes a cycle
+struct WeightPlan {
+    tc::Tile tile;
+    int slabs;
+    long long tiles(const ai2b_dense *d) const
+    {
+        return (long long)((d->outer + tile.rows() - 1) / tile.rows()) * ((d->inner + tile.columns - 1) / tile.columns);
+    }
+};
+static WeightPlan plan_weight(const ai2b_dense *d)
+{
+    WeightPlan best{{64, false}, 1};
+    double least = 1e300;
+    const double stages = d->rows / (double)tc::BK + 0.5 * d->groups;
+    for (int bn = 64; bn <= (d->dtype == AI2B_F32 ? 128 : 256); bn *= 2)
+        for (int pair = 0; pair < (bn == 64 ? 1 : 2); pair++) {
+            WeightPlan p{{bn, pair != 0}, 1};
+            const double tiles = (double)p.tiles(d), units = sm_count() / (pair ? 2 : 1), stage = tc::stage_cost(p.tile, planes_of(d->dtype));
+            for (; p.slabs <= 4 * sm_count() && p.slabs * WeightLine::LEAST < stages + WeightLine::LEAST; p.slabs++) {
+                const double rounds = (double)(long long)((p.slabs * tiles + units - 1) / units);
+                const double cost = rounds * (stages / p.slabs * stage + 22.0 * bn) + (p.slabs + d->groups) * tiles * p.tile.rows() * bn * 8 / 3400 + (pair ? 2000.0 : 0.0);
+                if (cost < least) {
+                    least = cost;
+                    best = p;
+                }
+            }
+        }
+    return best;
+}
+
 struct BackwardPlan {
     bool tensor, slopes;
     int weight_height, bias_height, vectors;
-    tc::Tile weight_tile;
+    WeightPlan weight_plan;
     PackedRows gz, x, weight;     // gz.copy: made by slope_kernel
     size_t weight_part, bias_part, total;
 };
@@ -811,14 +966,8 @@ static BackwardPlan plan_backward(const ai2b_dense *d)
     BackwardPlan p{};
     p.tensor = backward_on_tensor_cores(d);
     p.slopes = d->activation != AI2B_ACT_NONE;
-    if (p.tensor) {
-        // tiles of a slab of 2048 rows, as many slabs as there are
-        p.weight_tile = tc::best_tile(planes_of(d->dtype), d->outer, 0, d->inner, (d->rows + 2047) / 2048, 2048, sm_count());
-        const int bm = p.weight_tile.rows(), bn = p.weight_tile.columns;
-        p.weight_height = slab_height(d->rows, (long long)((d->outer + bm - 1) / bm) * ((d->inner + bn - 1) / bn) * (p.weight_tile.pair ? 2 : 1), 2, 256);
-    } else {
-        p.weight_height = slab_height(d->rows, (long long)((d->outer + FT - 1) / FT) * ((d->inner + FT - 1) / FT), 2, 256);
-    }
+    if (p.tensor) p.weight_plan = plan_weight(d);
+    else p.weight_height = slab_height(d->rows, (long long)((d->outer + FT - 1) / FT) * ((d->inner + FT - 1) / FT), 2, 256);
     p.vectors = slope_vectors(d);
     p.bias_height = slab_height(d->rows, (d->outer + 32 * p.vectors - 1) / (32 * p.vectors), 8, 64);
     if (p.tensor) {
@@ -833,7 +982,12 @@ static BackwardPlan plan_backward(const ai2b_dense *d)
         }
     }
     p.weight_part = p.total;
-    p.total += round256(sizeof(float) * (size_t)slab_bound(d->rows, p.weight_height, d->groups) * d->outer * d->inner);
+    if (p.tensor) {
+        const tc::Tile t = p.weight_plan.tile;
+        p.total += round256(sizeof(float) * (size_t)(d->groups + p.weight_plan.slabs) * p.weight_plan.tiles(d) * t.rows() * t.columns);
+    } else {
+        p.total += round256(sizeof(float) * (size_t)slab_bound(d->rows, p.weight_height, d->groups) * d->outer * d->inner);
+    }
     p.bias_part = p.total;
     p.total += round256(sizeof(float) * (size_t)slab_bound(d->rows, p.bias_height, d->groups) * d->outer);
     return p;
@@ -899,10 +1053,10 @@ static int multiply_rows(const ai2b_dense *d, const PackedRows &a, const PackedR
 }
 
 template <typename T>
-static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const unsigned char *ws, float *part, cudaStream_t st)
+static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const unsigned char *ws, float *part, WeightLine *line, cudaStream_t st)
 {
     constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
-    return tc::with_tile<PLANES == 1 ? 256 : 128>(p.weight_tile, [&](auto bn, auto pair) {
+    return tc::with_tile<PLANES == 1 ? 256 : 128>(p.weight_plan.tile, [&](auto bn, auto pair) {
         constexpr int BN = decltype(bn)::value;
         constexpr bool PAIR = decltype(pair)::value;
         tc::Operands ops{};
@@ -912,10 +1066,15 @@ static int multiply_weight(const ai2b_dense *d, const BackwardPlan &p, const uns
         if (rc != AI2B_OK) return rc;
         ops.a_stack = ops.b_stack = 1;
         ops.is_bf16 = d->dtype != AI2B_F16;
-        const int tile_rows = p.weight_tile.rows();
-        const WeightItems<BN> items{{d->d_offsets, d->groups, p.weight_height, d->rows}, tile_rows, (d->outer + tile_rows - 1) / tile_rows, (d->inner + BN - 1) / BN, d->outer};
-        const WeightOut out{part, d->inner, d->outer, d->inner % 4 == 0};
-        return tc::launch<PLANES, BN, PAIR, true, true>(ops, items, out, slab_bound(d->rows, p.weight_height, d->groups) * items.row_tiles * items.column_tiles, st);
+        const int tile_rows = p.weight_plan.tile.rows(), tiles = (int)p.weight_plan.tiles(d);
+        int units = 0;
+        rc = tc::units<PLANES, BN, PAIR, true, true, WeightItems<BN>, WeightOut>(&units);
+        if (rc != AI2B_OK) return rc;
+        const long long all = (long long)tiles * p.weight_plan.slabs;
+        *line = WeightLine{d->d_offsets, d->groups, tiles, p.weight_plan.slabs, (int)(all < units ? all : units), d->rows};
+        const WeightItems<BN> items{*line, tile_rows, (d->inner + BN - 1) / BN, d->outer};
+        const WeightOut out{part, d->inner, tile_rows, BN};
+        return tc::launch<PLANES, BN, PAIR, true, true>(ops, items, out, line->units, st);
     });
 }
 
@@ -1047,9 +1206,10 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
                 AI2B_CUDA(p.gz.copy ? go(rows_fma_kernel<T, float>, (const float *)gz) : go(rows_fma_kernel<T, T>, (const T *)gz));
             }
         }
+        WeightLine line{};
         if (d->d_gweight) {
             if (p.tensor) {
-                const int rc2 = multiply_weight<T>(d, p, ws, wpart, st);
+                const int rc2 = multiply_weight<T>(d, p, ws, wpart, &line, st);
                 if (rc2 != AI2B_OK) return rc2;
             } else if (d->rows > 0) {
                 const dim3 grid((unsigned)slab_bound(d->rows, p.weight_height, d->groups), (d->outer + FT - 1) / FT, (d->inner + FT - 1) / FT);
@@ -1061,16 +1221,23 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
             }
         }
         if (d->d_gweight || d->d_gbias) {
+            // as many blocks as are resident: each finds its group's place on the line first, which takes as long as some thousand sums
+            const int most = 8 * sm_count() / d->groups > 1 ? 8 * sm_count() / d->groups : 1;
             auto job = [&](void *to, const float *part, long long size, int height) {
-                const long long blocks = to ? (size + 1023) / 1024 : 0;
-                return SlabSum<T>{(T *)to, part, size, slab_bound(d->rows, height, d->groups), height, (int)(blocks < 2048 ? blocks : 2048)};
+                const long long blocks = to ? (size + 255) / 256 : 0;
+                return SlabSum<T>{(T *)to, part, size, slab_bound(d->rows, height, d->groups), height, (int)(blocks < most ? blocks : most)};
             };
-            const SlabSum<T> w = job(d->d_gweight, wpart, (long long)d->outer * d->inner, p.weight_height), b = job(d->d_gbias, bpart, d->outer, p.bias_height);
-            const dim3 grid(w.blocks + b.blocks, d->groups);
-            const bool fours = (d->d_gweight ? d->outer * (long long)d->inner % 4 == 0 : true) && d->outer % 4 == 0 &&
-                               common_alignment(d->d_gweight, d->d_gbias) >= 4 * (int)sizeof(T);
-            if (fours) AI2B_CUDA(launch_chained(sum_slabs_kernel<T, 4>, grid, dim3(256), 0, st, w, b, d->d_offsets, d->rows));
-            else AI2B_CUDA(launch_chained(sum_slabs_kernel<T, 1>, grid, dim3(256), 0, st, w, b, d->d_offsets, d->rows));
+            const SlabSum<T> b = job(d->d_gbias, bpart, d->outer, p.bias_height);
+            if (p.tensor) {
+                const int rows = p.weight_plan.tile.rows(), columns = p.weight_plan.tile.columns;
+                const long long blocks = d->d_gweight ? ((long long)line.tiles * rows * columns + 1023) / 1024 : 0;
+                const PieceSum<T> w{(T *)d->d_gweight, wpart, line, rows, columns, (d->inner + columns - 1) / columns, d->outer, d->inner, (int)(blocks < most ? blocks : most),
+                                    common_alignment(d->d_gweight, (long long)sizeof(T) * d->inner) >= 4 * (int)sizeof(T)};
+                AI2B_CUDA(launch_chained(sum_pieces_kernel<T>, dim3(w.blocks + b.blocks, d->groups), dim3(256), 0, st, w, b, d->d_offsets, d->rows));
+            } else {
+                const SlabSum<T> w = job(d->d_gweight, wpart, (long long)d->outer * d->inner, p.weight_height);
+                AI2B_CUDA(launch_chained(sum_slabs_kernel<T>, dim3(w.blocks + b.blocks, d->groups), dim3(256), 0, st, w, b, d->d_offsets, d->rows));
+            }
         }
         return (int)AI2B_OK;
     });

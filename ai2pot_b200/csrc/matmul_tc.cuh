@@ -157,6 +157,7 @@ struct Item {
     long long row, row_end;       // rows and first column of the result
     int col, batch;
     int mirror_from;              // results that are their own transpose: tiles from this column on are stored twice
+    long long cursor;             // of Items, from one call to the next
 };
 
 template <int PLANES, int BN, bool PAIR>
@@ -203,7 +204,7 @@ struct Operands {
 };
 
 // Items::prepare(table), by all threads, may leave something in shared memory; Items::get(table, t, item), by whole warps, gives tile t, false after
-// the last one. (table is NULL, and nothing was prepared, where there is no room for it.) Out takes 32 x 32 sums at a time, in shared memory:
+// the last one; it may keep a cursor in the item, -1 at first. (table is NULL, and nothing was prepared, where there is no room for it.) Out takes 32 x 32 sums at a time, in shared memory:
 // out.load(ahead, item, first row, first column, lane) reads what it needs of memory, out(item, first row, first column, sums, lane, ahead, dry) stores;
 // dry: one pass through its code, with no access to memory.
 template <int PLANES, int BN, bool PAIR, bool A_MN, bool B_MN, typename Items, typename Out>
@@ -280,7 +281,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
 
     bool ok = true;
     if (warp == 0) {
-        Item it;
+        Item it{};
+        it.cursor = -1;
         unsigned issued = 0;             // stages started
         for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
             const int a_at = it.a_at + rank * BM, b_at = it.b_at + rank * S::B_ROWS;
@@ -311,7 +313,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
         }
     } else if (warp == 1) {
         const unsigned idesc = instruction_descriptor(ops.is_bf16, A_MN, B_MN, BM * S::BLOCKS, BN);
-        Item it;
+        Item it{};
+        it.cursor = -1;
         unsigned used = 0, sets = 0, tails = 0;          // stages and sets of accumulators begun; a bit per stage, turned over by its ragged uses
         for (long long t = first_tile; ok && items.get(table, t, it); t += tile_step) {
             for (int k0 = it.k_begin; ok && k0 < it.k_end; k0 = k0 < it.k_end - S::CHUNK ? k0 + S::CHUNK : it.k_end) {
@@ -386,7 +389,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
     } else {
         const int quarter = warp & 3, share = (warp - 2) >> 2;      // rows 32 * quarter.., columns 32 * share.. of every 32 * SHARES
         float *mine = staging + (warp - 2) * 1024;
-        Item it;
+        Item it{};
+        it.cursor = -1;
         unsigned sets = 0;
         // Lane l holds row l of 32 sums: through shared memory, so that neighbouring lanes get neighbouring columns. Four columns at a time, permuted
         // within the row, keep both directions free of bank conflicts.
@@ -402,7 +406,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
         // caches while the first products are under way; fetching it then, line after line, took 4,400 cycles of a tile of 128 x 128.
         bool dry = true;
         for (long long t = first_tile; ok;) {
-            if (dry) it = Item{0, 0, 0, 0, 0, 0, 0, 32 * (long long)(quarter + 1) + rank * BM, 0, 0, 0};
+            if (dry) it = Item{0, 0, 0, 0, 0, 0, 0, 32 * (long long)(quarter + 1) + rank * BM, 0, 0, 0, -1};
             else if (!items.get(table, t, it)) break;
             const long long row = it.row + rank * BM + 32 * quarter;
             constexpr int PARTS = (BN + 32 * S::SHARES - 1) / (32 * S::SHARES);
@@ -534,20 +538,29 @@ int resident_pairs(KernelSetup &ks, Kern kern, int threads, size_t smem, int *pa
     return AI2B_OK;
 }
 
+// Blocks (pairs) that run at once
 template <int PLANES, int BN, bool PAIR, bool A_MN, bool B_MN, typename Items, typename Out>
-int launch(const Operands &ops, const Items &items, const Out &out, long long tiles, cudaStream_t st)
+int units(int *n)
 {
     using S = Shape<PLANES, BN, PAIR>;
     auto kern = product_kernel<PLANES, BN, PAIR, A_MN, B_MN, Items, Out>;
     static KernelSetup ks;
     const int rc = kernel_setup(ks, kern, S::SMEM);
     if (rc != AI2B_OK) return rc;
-    int units = sm_count();
-    if constexpr (PAIR) {
-        const int rc2 = resident_pairs(ks, kern, S::THREADS, S::SMEM, &units);
-        if (rc2 != AI2B_OK) return rc2;
-    }
-    AI2B_CUDA(launch_chained(kern, dim3((unsigned)(tiles < units ? tiles : units) * S::BLOCKS), dim3(S::THREADS), S::SMEM, st, ops, items, out));
+    if constexpr (PAIR) return resident_pairs(ks, kern, S::THREADS, S::SMEM, n);
+    *n = sm_count();
+    return AI2B_OK;
+}
+
+template <int PLANES, int BN, bool PAIR, bool A_MN, bool B_MN, typename Items, typename Out>
+int launch(const Operands &ops, const Items &items, const Out &out, long long tiles, cudaStream_t st)
+{
+    using S = Shape<PLANES, BN, PAIR>;
+    int n = 0;
+    const int rc = units<PLANES, BN, PAIR, A_MN, B_MN, Items, Out>(&n);
+    if (rc != AI2B_OK) return rc;
+    AI2B_CUDA(launch_chained(product_kernel<PLANES, BN, PAIR, A_MN, B_MN, Items, Out>, dim3((unsigned)(tiles < n ? tiles : n) * S::BLOCKS), dim3(S::THREADS), S::SMEM, st, ops, items,
+                             out));
     return AI2B_OK;
 }
 
@@ -559,17 +572,21 @@ struct Tile {
     int b_rows() const { return pair ? columns / 2 : columns; }      // box of a K-major B
 };
 
+// Cycles of a stage: the longer of its products and of its copies at 58 bytes a cycle
+inline double stage_cost(Tile t, int planes)
+{
+    const double products = 2.0 * t.columns * (planes * (planes + 1) / 2), copies = planes * 128.0 * (BM + t.b_rows()) / 58.0;
+    return products > copies ? products : copies;
+}
+
 // What the products of `rows` x `columns` results (`matrices` of them; `edges` more tiles of rows that are not full) would take in tiles of
-// one kind, in cycles: per stage the longer of its products and of its copies at 58 bytes a cycle; a tile's last stage and its epilogue (22 cycles a
-// column) are not overlapped by another of the same block.
+// one kind, in cycles; a tile's last stage and its epilogue (22 cycles a column) are not overlapped by another of the same block.
 inline double tile_cost(Tile t, int planes, long long rows, long long edges, long long columns, long long matrices, long long inner, int sms)
 {
-    const int terms = planes * (planes + 1) / 2;
-    const double products = 2.0 * t.columns * terms, copies = planes * 128.0 * (BM + t.b_rows()) / 58.0;
     const double tiles = (double)matrices * (double)((rows + t.rows() - 1) / t.rows() + edges) * (double)((columns + t.columns - 1) / t.columns);
     const double waves = (double)(long long)((tiles + sms / (t.pair ? 2 : 1) - 1) / (sms / (t.pair ? 2 : 1)));
     const double stages = (double)((inner + BK - 1) / BK), epilogue = 22.0 * t.columns;
-    const double tile = stages * (products > copies ? products : copies);
+    const double tile = stages * stage_cost(t, planes);
     return waves * (tile > epilogue ? tile : epilogue) + epilogue + (t.pair ? 3500.0 : 1500.0);      // (a pair waits for both blocks)
 }
 // The kind that takes least. (Planes need two accumulators for each of two tiles: 128 columns at most.)
