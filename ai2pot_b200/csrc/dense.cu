@@ -604,8 +604,8 @@ struct RowOut {
                 const long long at = row + r;
                 const bool two = r + 1 < last && !dry;
                 float2 z;
-                z.x = mine[32 * r + 4 * ((lane / 4) ^ (r & 7)) + lane % 4] + bias;
-                z.y = mine[32 * (r + 1) + 4 * ((lane / 4) ^ ((r + 1) & 7)) + lane % 4] + bias;
+                z.x = tc::staged_one(mine, r, lane) + bias;
+                z.y = tc::staged_one(mine, r + 1, lane) + bias;
                 Activated2 a = finish<ACT, SLOPE>(z);
                 if (add) {
                     a.value.x += to_float(o.residual[at * o.residual_stride + col]);

@@ -148,6 +148,12 @@ __host__ __device__ constexpr unsigned instruction_descriptor(bool is_bf16, bool
     return 1u << 4 | (is_bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (unsigned)(n >> 3) << 17 | (unsigned)(m >> 4) << 24;
 }
 
+// Where columns [4 i, 4 i + 4) of row r of a warp's 32 x 32 sums lie in its staging memory: permuted within the row, so that rows by lanes and pieces of rows
+// are free of bank conflicts
+__device__ __forceinline__ int staged_at(int r, int i) { return 32 * r + 4 * (i ^ (r & 7)); }
+__device__ __forceinline__ float4 staged(const float *mine, int r, int i) { return *reinterpret_cast<const float4 *>(mine + staged_at(r, i)); }
+__device__ __forceinline__ float staged_one(const float *mine, int r, int c) { return mine[staged_at(r, c >> 2) + (c & 3)]; }
+
 // ---- a tile of work -------------------------------------------------------------------------------------------------------
 
 struct Item {
@@ -392,12 +398,11 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
         Item it{};
         it.cursor = -1;
         unsigned sets = 0;
-        // Lane l holds row l of 32 sums: through shared memory, so that neighbouring lanes get neighbouring columns. Four columns at a time, permuted
-        // within the row, keep both directions free of bank conflicts.
+        // Lane l holds row l of 32 sums: through shared memory, so that neighbouring lanes get neighbouring columns.
         auto hand_over = [&](const float (&v)[32], long long row, int col, const typename Out::Ahead &ahead, bool dry) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                *reinterpret_cast<float4 *>(mine + 32 * lane + 4 * (i ^ (lane & 7))) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                *reinterpret_cast<float4 *>(mine + staged_at(lane, i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             __syncwarp();
             out(it, row, col, mine, lane, ahead, dry);
             __syncwarp();
@@ -503,8 +508,6 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Shape<PLA
     }
 }
 
-// What an epilogue reads of a warp's 32 x 32 sums: columns [4 i, 4 i + 4) of row r
-__device__ __forceinline__ float4 staged(const float *mine, int r, int i) { return *reinterpret_cast<const float4 *>(mine + 32 * r + 4 * (i ^ (r & 7))); }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 

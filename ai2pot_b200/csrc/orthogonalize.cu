@@ -235,18 +235,30 @@ __device__ __forceinline__ void halves(float v, f16 &hi, f16 &lo)
     lo = __float2half_rn(v - __half2float(hi));
 }
 
-// X0 = G / (|G| + eps) as halves, rows padded to `stride`
-template <typename T>
+// X0 = G / (|G| + eps) as halves, rows padded to `stride`. A thread takes eight columns of a row; N: how many of them one access reads.
+template <typename T, int N>
 __global__ void __launch_bounds__(256) normalise_halves_kernel(f16 *__restrict__ hi, f16 *__restrict__ lo, long long stride, const T *__restrict__ g, int m, int n, int parts,
                                                                const double *__restrict__ part, double eps)
 {
     chain_wait();
     chain_release();
     const double scale = norm_scale(part + blockIdx.y * (long long)parts, parts, eps);
-    const long long size = (long long)m * n;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = row_of(i, n, size <= 0xffffffffLL), at = (blockIdx.y * (long long)m + r) * stride + (i - r * n);
-        halves((float)((double)to_float(g[blockIdx.y * size + i]) * scale), hi[at], lo[at]);
+    const int per_row = (int)(stride / 8);
+    const long long total = (long long)m * per_row;
+    const bool narrow = total <= 0xffffffffLL;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long r = row_of(i, per_row, narrow), row = blockIdx.y * (long long)m + r;
+        const int c = (int)(i - r * per_row) * 8;
+        Pack<f16, 8> h, l;
+#pragma unroll
+        for (int u = 0; u < 8; u += N) {
+            Pack<T, N> v{};
+            if (c + u < n) v = *reinterpret_cast<const Pack<T, N> *>(g + row * n + c + u);
+#pragma unroll
+            for (int j = 0; j < N; j++) halves((float)((double)to_float(v.v[j]) * scale), h.v[u + j], l.v[u + j]);
+        }
+        *reinterpret_cast<Pack<f16, 8> *>(hi + row * stride + c) = h;
+        *reinterpret_cast<Pack<f16, 8> *>(lo + row * stride + c) = l;
     }
 }
 
@@ -318,7 +330,7 @@ struct BatchOut {
 #pragma unroll 2
             for (int r = 0; r < last; r++) {
                 const long long at = (matrix + row + r) * stride + col;
-                float v = beta * mine[32 * r + 4 * ((lane / 4) ^ (r & 7)) + lane % 4];
+                float v = beta * tc::staged_one(mine, r, lane);
                 if (dry) continue;
                 v = fmaf(alpha, __half2float(d_hi[at]) + __half2float(d_lo[at]), v);
                 result[(matrix + row + r) * columns + col] = from_float<T>(v * (1.f / SCALE));
@@ -345,11 +357,9 @@ struct BatchOut {
             for (int c = down; c < last; c += 8) {
                 d = next;
                 if (c + 8 < last) read(next, matrix + col0 + c + 8, col);
-                const float *from = mine + 32 * across + c % 4;
-                const int group = c / 4;
                 float2 s[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[j] = make_float2(from[64 * j + 4 * (group ^ (2 * j))], from[64 * j + 32 + 4 * (group ^ (2 * j + 1))]);
+                for (int j = 0; j < 4; j++) s[j] = make_float2(tc::staged_one(mine, across + 2 * j, c), tc::staged_one(mine, across + 2 * j + 1, c));
                 store(s, d, matrix + col0 + c, col, dry);
             }
         }
@@ -537,8 +547,13 @@ extern "C" int ai2b_orthogonalize(int dtype, void *d_out, const void *d_g, int b
                 return Halves{(f16 *)at, (f16 *)at + batch * rows * stride, rows, columns, stride};
             };
             const Halves x0 = halves_of(x, m, n), x1 = halves_of(next, m, n), g = halves_of(gram, s, s), q = halves_of(poly, s, s);
-            AI2B_CUDA(launch_chained(normalise_halves_kernel<T>, dim3(blocks, batch), dim3(256), 0, st, x0.hi, x0.lo, x0.stride, (const T *)d_g, m, n, parts, (const double *)norm,
-                                     eps));
+            constexpr int N = 16 / (int)sizeof(T);
+            const long long groups = (m * (x0.stride / 8) + 255) / 256, most = 8 * sm_count() / batch > 1 ? 8 * sm_count() / batch : 1;
+            const dim3 grid((unsigned)(groups < most ? groups : most), batch);
+            auto go = [&](auto kern) {
+                return launch_chained(kern, grid, dim3(256), 0, st, x0.hi, x0.lo, x0.stride, (const T *)d_g, m, n, parts, (const double *)norm, eps);
+            };
+            AI2B_CUDA(n % N == 0 && common_alignment(d_g) >= 16 ? go(normalise_halves_kernel<T, N>) : go(normalise_halves_kernel<T, 1>));
             constexpr int PLANES = std::is_same<T, bf16>::value ? 1 : 2;
             return m <= n ? iterate_tc<T, PLANES, true>((T *)d_out, x0, x1, g, q, steps, (float)a, (float)b, (float)c, batch, st)
                           : iterate_tc<T, PLANES, false>((T *)d_out, x0, x1, g, q, steps, (float)a, (float)b, (float)c, batch, st);
