@@ -917,7 +917,8 @@ static ForwardPlan plan_forward(const ai2b_dense *d)
 }
 
 // The tile of the weight gradient's products and the number of slabs that take least, in cycles: rounds of blocks, each as long as the stages of a slab and
-// an epilogue (22 cycles a column), and 8 bytes of every partial sum, written and read at 3400 bytes a cycle
+// an epilogue (22 cycles a column), and 8 bytes of every partial sum, written and read at 3400 bytes a cycle. As many slabs are looked at as one, two, three or four
+// rounds hold.
 struct WeightPlan {
     tc::Tile tile;
     int slabs;
@@ -935,9 +936,13 @@ static WeightPlan plan_weight(const ai2b_dense *d)
         for (int pair = 0; pair < (bn == 64 ? 1 : 2); pair++) {
             WeightPlan p{{bn, pair != 0}, 1};
             const double tiles = (double)p.tiles(d), units = sm_count() / (pair ? 2 : 1), stage = tc::stage_cost(p.tile, planes_of(d->dtype));
-            for (; p.slabs <= 4 * sm_count() && p.slabs * WeightLine::LEAST < stages + WeightLine::LEAST; p.slabs++) {
-                const double rounds = (double)(long long)((p.slabs * tiles + units - 1) / units);
-                const double cost = rounds * (stages / p.slabs * stage + 22.0 * bn) + (p.slabs + d->groups) * tiles * p.tile.rows() * bn * 8 / 3400 + (pair ? 2000.0 : 0.0);
+            const double most = stages / WeightLine::LEAST;
+            for (int round = 1; round <= 4; round++) {
+                double n = (double)(long long)(round * units / tiles);
+                n = n < 1 ? 1 : n > most ? (double)(long long)(most < 1 ? 1 : most) : n;
+                p.slabs = (int)n;
+                const double rounds = (double)(long long)((n * tiles + units - 1) / units);
+                const double cost = rounds * (stages / n * stage + 22.0 * bn) + (n + d->groups) * tiles * p.tile.rows() * bn * 8 / 3400 + (pair ? 2000.0 : 0.0);
                 if (cost < least) {
                     least = cost;
                     best = p;
@@ -1135,6 +1140,7 @@ extern "C" int ai2b_dense_forward(const ai2b_dense *d, void *stream)
     const ForwardPlan p = plan_forward(d);
     AI2B_REQUIRE(p.total == 0 || (d->d_workspace && d->workspace_bytes >= p.total), AI2B_ERR_WORKSPACE, "ai2b_dense_forward: workspace of %zu bytes, %zu needed",
                  d->workspace_bytes, p.total);
+    AI2B_REQUIRE(((size_t)d->d_workspace & 255) == 0, AI2B_ERR_WORKSPACE, "ai2b_dense_forward: the workspace is not aligned to 256 bytes");
     cudaStream_t st = (cudaStream_t)stream;
     unsigned char *ws = (unsigned char *)d->d_workspace;
     return with_type(d->dtype, [&](auto t) {
@@ -1161,9 +1167,10 @@ extern "C" int ai2b_dense_backward(const ai2b_dense *d, void *stream)
     const bool slopes = d->activation != AI2B_ACT_NONE;
     AI2B_REQUIRE(d->rows == 0 || d->d_gy, AI2B_ERR_INVALID, "ai2b_dense_backward: gy is NULL");
     AI2B_REQUIRE(d->gy_stride >= d->outer || d->rows <= 1, AI2B_ERR_INVALID, "ai2b_dense_backward: row stride %lld of gy is below %d", d->gy_stride, d->outer);
-    AI2B_REQUIRE(!slopes || d->rows == 0 || d->d_slope, AI2B_ERR_INVALID, "ai2b_dense_backward: the slopes that the forward call kept are NULL");
+    AI2B_REQUIRE(!slopes || d->rows == 0 || d->d_slope || !(d->d_gx || d->d_gweight || d->d_gbias), AI2B_ERR_INVALID, "ai2b_dense_backward: the slopes that the forward call kept are NULL");
     const BackwardPlan p = plan_backward(d);
     AI2B_REQUIRE(d->d_workspace && d->workspace_bytes >= p.total, AI2B_ERR_WORKSPACE, "ai2b_dense_backward: workspace of %zu bytes, %zu needed", d->workspace_bytes, p.total);
+    AI2B_REQUIRE(((size_t)d->d_workspace & 255) == 0, AI2B_ERR_WORKSPACE, "ai2b_dense_backward: the workspace is not aligned to 256 bytes");
     cudaStream_t st = (cudaStream_t)stream;
     unsigned char *ws = (unsigned char *)d->d_workspace;
     return with_type(d->dtype, [&](auto t) {

@@ -518,6 +518,7 @@ extern "C" int ai2b_orthogonalize(int dtype, void *d_out, const void *d_g, int b
     AI2B_REQUIRE(d_out && d_g, AI2B_ERR_INVALID, "ai2b_orthogonalize: NULL pointer");
     const OrthogonalizePlan p = plan_orthogonalize(batch, m, n);
     AI2B_REQUIRE(d_workspace && workspace_bytes >= p.total, AI2B_ERR_WORKSPACE, "ai2b_orthogonalize: workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
+    AI2B_REQUIRE(((size_t)d_workspace & 255) == 0, AI2B_ERR_WORKSPACE, "ai2b_orthogonalize: the workspace is not aligned to 256 bytes");
     cudaStream_t st = (cudaStream_t)stream;
     unsigned char *ws = (unsigned char *)d_workspace;
     return with_type(dtype, [&](auto t) {

@@ -593,7 +593,8 @@ int ai2b_chained_copy(void *dst, const void *src, size_t bytes, void *stream);
 /* ------------------------------------------------------------------------------------------
  * Fitting networks: the pieces of per-species networks (or of a mixture of networks) over the descriptors of the calls above. The
  * reference has per-type fitting networks in its deepmd and nn-MTP models (ai2pot/models/deepmd/se_r.py, source/descriptor/nnmtp).
- * Element types: AI2B_F32, AI2B_BF16 or AI2B_F16 for x, weights and results of a call alike; sums are float.
+ * Element types: AI2B_F32, AI2B_BF16 or AI2B_F16 for x, weights and results of a call alike; sums are float. Workspaces are aligned
+ * to 256 bytes, arrays to their elements.
  * ---------------------------------------------------------------------------------------- */
 #define AI2B_F32 0
 #define AI2B_BF16 1

@@ -49,7 +49,8 @@ def test_dense_refusals():
                                (dict(x_stride=3), -1, b"row stride 3"), (dict(d_weight=None), -1, b"weight is NULL"), (dict(d_y=None), -1, b"y is NULL"),
                                (dict(d_residual=256, residual_stride=2), -1, b"residual")]:
         refused(lib.ai2b_dense_forward(C.byref(Dense(**dict(good, **change))), NULL), code, text)
-    for change, code, text in [(dict(d_gy=None), -1, b"gy is NULL"), (dict(gy_stride=1), -1, b"row stride 1"), (dict(d_slope=None), -1, b"slopes"), (dict(), -4, b"workspace")]:
+    for change, code, text in [(dict(d_gy=None), -1, b"gy is NULL"), (dict(gy_stride=1), -1, b"row stride 1"), (dict(d_slope=None, d_gx=256), -1, b"slopes"), (dict(), -4, b"workspace"),
+                               (dict(d_workspace=264, workspace_bytes=1 << 40), -4, b"aligned")]:
         refused(lib.ai2b_dense_backward(C.byref(Dense(**dict(good, **change))), NULL), code, text)
     refused(lib.ai2b_dense_forward(NULL, NULL), -1, b"NULL description")
 

@@ -248,6 +248,46 @@ def test_gradients_of_some_inputs_only():
         assert torch.equal(g, full["g" + key]), key
 
 
+@pytest.mark.parametrize("key", ["x", "weight", "bias", "residual"])
+def test_gradients_of_some_inputs_of_groups(key):
+    """One input's gradient alone, rows of no network at the end: the residual's needs no slopes, which are not kept then."""
+    offsets = torch.tensor([0, 90, 90, 180], device="cuda").int()
+    t, gy = make(200, 3, 64, 48, torch.bfloat16)
+    full = run(t, "tanh", offsets, gy)
+    leaves = {k2: v.detach().requires_grad_(k2 == key) for k2, v in t.items()}
+    y = fitnet.dense(leaves["x"], leaves["weight"], leaves["bias"], leaves["residual"], "tanh", offsets)
+    g, = torch.autograd.grad(y, leaves[key], gy)
+    assert torch.equal(g, full["g" + key])
+
+
+def test_recorded_in_a_graph():
+    """Layers, routing and updates recorded once and replayed on other values give the results of direct calls."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    types = torch.randint(-1, 3, (2000,), generator=g, device="cuda", dtype=torch.int32)
+    x, w = torch.randn(2000, 96, generator=g, device="cuda"), torch.randn(3, 160, 96, generator=g, device="cuda") * 0.1
+    ones = torch.ones(2000, 1, device="cuda")
+
+    def call():
+        route = fitnet.route(types, 3)
+        h = fitnet.dense(fitnet.dispatch(x, route), w, activation="gelu", offsets=route.offsets)
+        return fitnet.combine(h, ones, route), fitnet.orthogonalize(w)
+
+    with torch.no_grad():
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        for seed in (1, 2):
+            g.manual_seed(seed)
+            x.copy_(torch.randn(2000, 96, generator=g, device="cuda"))
+            types.copy_(torch.randint(-1, 3, (2000,), generator=g, device="cuda", dtype=torch.int32))
+            w.copy_(torch.randn(3, 160, 96, generator=g, device="cuda") * 0.1)
+            graph.replay()
+            want = call()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
 def test_refusals():
     t, gy = make(20, 3, 8, 12, torch.float32)
     offsets = torch.tensor([0, 5, 10, 20]).int().cuda()

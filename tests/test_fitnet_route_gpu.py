@@ -98,6 +98,12 @@ def test_strides_and_alignment(dtype):
         check_all(index, *run_all(index, 4, 48, dtype, x_view=view))
 
 
+def test_no_tokens():
+    index = torch.zeros(0, 2, dtype=torch.int32)
+    inputs, out = run_all(index, 3, 8, torch.float32)
+    assert out["xs"].shape == (0, 8) and out["y"].shape == (0, 8) and out["gw"].shape == (0, 2) and out["gys"].shape == (0, 8)
+
+
 def test_dropped_slots_do_not_read_what_they_hold():
     """Weights and rows of dropped slots may hold anything: neither sums nor gradients see them."""
     index = torch.tensor([[0, -1], [-1, -1], [1, 0]], dtype=torch.int32)
