@@ -582,26 +582,32 @@ inline double stage_cost(Tile t, int planes)
     return products > copies ? products : copies;
 }
 
-// What the products of `rows` x `columns` results (`matrices` of them; `edges` more tiles of rows that are not full) would take in tiles of
-// one kind, in cycles; a tile's last stage and its epilogue (22 cycles a column) are not overlapped by another of the same block.
-inline double tile_cost(Tile t, int planes, long long rows, long long edges, long long columns, long long matrices, long long inner, int sms)
+// A product whose tile is to be chosen: `matrices` results of `rows` x `columns`, `edges` more tiles of rows that are not full; epilogue: how long one takes
+// against that of a 16-bit layer; share: of the tiles that is multiplied (half, where the result is its own transpose)
+struct Extent {
+    int planes;
+    double rows, columns, inner, matrices, edges, epilogue, share;
+};
+
+// What it takes in tiles of one kind, in cycles. A tile takes as long as its stages or its epilogue, whichever is longer; the last one's epilogue is not
+// overlapped. Epilogues by measurement (silu, 13824 x 128 x 1024): 4,700 cycles for 64 columns of 16 bits, 6,500 for 128, 11,400 for 256.
+inline double tile_cost(Tile t, const Extent &e, int sms)
 {
-    const double tiles = (double)matrices * (double)((rows + t.rows() - 1) / t.rows() + edges) * (double)((columns + t.columns - 1) / t.columns);
-    const double waves = (double)(long long)((tiles + sms / (t.pair ? 2 : 1) - 1) / (sms / (t.pair ? 2 : 1)));
-    const double stages = (double)((inner + BK - 1) / BK), epilogue = 22.0 * t.columns;
-    const double tile = stages * stage_cost(t, planes);
+    const double units = sms / (t.pair ? 2 : 1), row_tiles = (double)(long long)((e.rows + t.rows() - 1) / t.rows()) + e.edges;
+    const double tiles = e.matrices * e.share * row_tiles * (double)(long long)((e.columns + t.columns - 1) / t.columns);
+    const double waves = (double)(long long)((tiles + units - 1) / units), epilogue = e.epilogue * (2500.0 + 33.0 * t.columns);
+    const double tile = (double)(long long)((e.inner + BK - 1) / BK) * stage_cost(t, e.planes);
     return waves * (tile > epilogue ? tile : epilogue) + epilogue + (t.pair ? 3500.0 : 1500.0);      // (a pair waits for both blocks)
 }
 // The kind that takes least. (Planes need two accumulators for each of two tiles: 128 columns at most.)
-inline Tile best_tile(int planes, long long rows, long long edges, long long columns, long long matrices, long long inner, int sms)
+inline Tile best_tile(const Extent &e, int sms)
 {
     Tile best{64, false};
     double least = 1e300;
-    for (int bn = 64; bn <= (planes > 1 ? 128 : 256); bn *= 2)
-        for (int pair = 0; pair < 2; pair++) {
-            if (pair && bn == 64) continue;
+    for (int bn = 64; bn <= (e.planes > 1 ? 128 : 256); bn *= 2)
+        for (int pair = 0; pair < (bn == 64 ? 1 : 2); pair++) {
             const Tile t{bn, pair != 0};
-            const double cost = tile_cost(t, planes, rows, edges, columns, matrices, inner, sms);
+            const double cost = tile_cost(t, e, sms);
             if (cost < least) {
                 least = cost;
                 best = t;

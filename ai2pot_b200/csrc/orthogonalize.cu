@@ -453,7 +453,8 @@ struct Halves {
 template <int PLANES, bool A_MN, bool B_MN, typename Out>
 static int product_tc(const Halves &a, const Halves &b, const Out &out, int inner, int batch, cudaStream_t st)
 {
-    tc::Tile tile = tc::best_tile(PLANES, out.rows, 0, out.columns, batch, inner, sm_count());
+    // (halves added to the sums and stored twice take twice as long as a layer's epilogue)
+    tc::Tile tile = tc::best_tile({PLANES, (double)out.rows, (double)out.columns, (double)inner, (double)batch, 0.0, 2.0, out.symmetric ? 0.5 : 1.0}, sm_count());
     // half of a symmetric result is not multiplied: tiles are square, or two to a square
     if (out.symmetric && tile.columns > tile.rows()) tile.columns = tile.rows();
     if (out.symmetric && tile.columns < 128) tile.columns = 128;
