@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(256) slope_kernel(void *__restrict__ gz, long 
             }
         }
     }
-    if (!part || !kept) return;
+    if (!part || !kept || blockIdx.x + 1 == gridDim.x) return;      // (the last block has no slab of a group, unless the offsets do not ascend)
 #pragma unroll
     for (int n = 0; n < N; n++) sums[warp][lane * N + n] = sum[n];
     __syncthreads();
@@ -425,7 +425,7 @@ struct SlabSum {
     long long size, slabs;        // of one group's result; slabs that part has room for
     int height, blocks;           // blocks of the grid's x that belong to it
 };
-template <typename T, int N>
+template <typename T>
 __device__ __forceinline__ void sum_slabs(const SlabSum<T> &j, int block, int e, const int *offsets, long long rows, long long *shared)
 {
     if (threadIdx.x < 32) {
@@ -437,18 +437,11 @@ __device__ __forceinline__ void sum_slabs(const SlabSum<T> &j, int block, int e,
     // (`slabs` are there, whatever the offsets say)
     const int n = (int)min(tiles_of(r.end - r.begin, j.height), j.slabs - shared[0]);
     const float *part = j.part + shared[0] * j.size;
-    for (long long i = ((long long)block * blockDim.x + threadIdx.x) * N; i < j.size; i += (long long)j.blocks * blockDim.x * N) {
-        float sum[N] = {};
+    for (long long i = (long long)block * blockDim.x + threadIdx.x; i < j.size; i += (long long)j.blocks * blockDim.x) {
+        float sum = 0.f;
 #pragma unroll 4
-        for (int s = 0; s < n; s++) {
-            const Pack<float, N> v = *reinterpret_cast<const Pack<float, N> *>(part + s * j.size + i);
-#pragma unroll
-            for (int c = 0; c < N; c++) sum[c] += v.v[c];
-        }
-        Pack<T, N> out;
-#pragma unroll
-        for (int c = 0; c < N; c++) out.v[c] = from_float<T>(sum[c]);
-        *reinterpret_cast<Pack<T, N> *>(j.out + e * j.size + i) = out;
+        for (int s = 0; s < n; s++) sum += part[s * j.size + i];
+        j.out[e * j.size + i] = from_float<T>(sum);
     }
 }
 template <typename T>
@@ -457,8 +450,8 @@ __global__ void __launch_bounds__(256) sum_slabs_kernel(SlabSum<T> a, SlabSum<T>
     __shared__ long long shared[1];
     chain_wait();
     chain_release();
-    if ((int)blockIdx.x < a.blocks) sum_slabs<T, 1>(a, blockIdx.x, blockIdx.y, offsets, rows, shared);
-    else sum_slabs<T, 1>(b, blockIdx.x - a.blocks, blockIdx.y, offsets, rows, shared);
+    if ((int)blockIdx.x < a.blocks) sum_slabs<T>(a, blockIdx.x, blockIdx.y, offsets, rows, shared);
+    else sum_slabs<T>(b, blockIdx.x - a.blocks, blockIdx.y, offsets, rows, shared);
 }
 
 // ---- products on the tensor cores -------------------------------------------------------------------------------------------
@@ -788,7 +781,6 @@ struct WeightItems {
 struct WeightOut {
     float *part;              // [slot][tile_rows][tile_columns]
     int columns, tile_rows, tile_columns;
-    static constexpr bool BY_ROWS = false;
     struct Ahead {};
     __device__ __forceinline__ void load(Ahead &, const tc::Item &, long long, int, int) const {}
     __device__ __forceinline__ void operator()(const tc::Item &it, long long row, int col0, const float *mine, int lane, const Ahead &, bool dry) const
@@ -817,7 +809,7 @@ __global__ void __launch_bounds__(256) sum_pieces_kernel(PieceSum<T> w, SlabSum<
     chain_wait();
     chain_release();
     if ((int)blockIdx.x >= w.blocks) {
-        sum_slabs<T, 1>(b, blockIdx.x - w.blocks, blockIdx.y, offsets, rows, shared);
+        sum_slabs<T>(b, blockIdx.x - w.blocks, blockIdx.y, offsets, rows, shared);
         return;
     }
     const int e = blockIdx.y;

@@ -8,7 +8,8 @@
 //   combine  y[t] = sum_j w[t,j] ys[position[t,j]]                  (sums in float, j ascending: no atomics, same bits every time)
 //   combine's gradient  gys[position[s]] = w[s] gy[t], gw[s] = <gy[t], ys[position[s]]>, zero for dropped slots and rows
 //
-// All of it moves bytes: each row is read and written once, in accesses of up to 16 bytes by neighbouring lanes.
+// All of it moves bytes: each row is read and written once, in accesses of up to 16 bytes by neighbouring lanes. 1,048,576 x 64 floats in four networks:
+// plan 13 us (two passes over the index), dispatch 85 us (6.3 TB/s), combination 100 us (5.4 TB/s).
 #include "fitnet.cuh"
 
 namespace ai2b {
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(V *__restrict__ out, cons
 }
 
 // TOKENS accesses of different tokens and SLOTS of a token's slots are in flight at once: four in all, so that the rows of a token with one
-// slot do not wait for one another (1,048,576 x 64 floats: 145 us with one, 84 with four).
+// slot do not wait for one another (1,048,576 x 64 floats: 145 us with one, 100 with four; its bytes take 84).
 template <typename T, int N, int TOKENS, int SLOTS>
 __global__ void __launch_bounds__(256) combine_kernel(Pack<T, N> *__restrict__ y, const Pack<T, N> *__restrict__ ys, long long ys_stride, const float *__restrict__ weights,
                                const int *__restrict__ position, long long tokens, int k, int per_row, long long rows)

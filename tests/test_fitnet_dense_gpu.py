@@ -306,3 +306,15 @@ def test_refusals():
     y = fitnet.dense(x.detach().requires_grad_(), w, offsets=offsets)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(y.sum(), y.grad_fn.next_functions[0][0].variable, create_graph=True)
+
+
+@pytest.mark.parametrize("values", [[0, -5, 2 ** 31 - 1, 40], [300, 200, 100, 0], [-2 ** 31, 250, 10, 260], [0, 300, 0, 300]])
+def test_offsets_that_do_not_ascend(values):
+    """Whatever offsets hold, no access leaves the rows and the workspace (results of such offsets have no meaning)."""
+    offsets = torch.tensor(values, device="cuda").int()
+    for inner, outer, dtype in [(24, 40, torch.float32), (256, 320, torch.bfloat16), (128, 136, torch.float32)]:
+        t, gy = make(300, 3, inner, outer, dtype)
+        leaves = {k: v.detach().requires_grad_() for k, v in t.items()}
+        y = fitnet.dense(leaves["x"], leaves["weight"], leaves["bias"], leaves["residual"], "tanh", offsets)
+        torch.autograd.grad(y, list(leaves.values()), gy)
+    torch.cuda.synchronize()

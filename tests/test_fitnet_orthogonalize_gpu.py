@@ -45,7 +45,7 @@ def check(g, got, steps=5, coefficients=MUON, eps=1e-7):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("batch,m,n", [(1, 1, 1), (1, 1, 7), (2, 9, 1), (3, 30, 20), (2, 17, 64), (1, 64, 64), (4, 65, 33), (2, 100, 300), (3, 128, 128), (1, 240, 240), (2, 257, 131),
-                                       (1, 500, 20), (8, 96, 160)])
+                                       (1, 500, 20), (8, 96, 160), (1, 3, 30000), (2, 20000, 4)])
 def test_shapes(batch, m, n, dtype):
     g = gradient_like(batch, m, n, dtype)
     check(g, fitnet.orthogonalize(g))
