@@ -7,7 +7,7 @@
 // An SM takes in about 58 bytes a cycle from L2 (measured: a stage of 24 KB in 410 cycles, whatever the products), and a stage of a 128 x 256 tile
 // has 96 for every cycle of its products. With PAIR two neighbouring blocks (a cluster) share a tile of 256 rows: each holds its 128 rows of A, half
 // of B's tile and the accumulators of its rows, and one thread of the first issues the products of both (cta_group::2). That is 64 bytes
-// a cycle for 256 x 256.
+// a cycle for 256 x 256. bfloat16 without an epilogue to speak of: 65536 x 1024 x 1024 in 105 us, 1.31 Pflop/s; 8192^3 in 786 us, 1.40 Pflop/s (a library product 650).
 //
 // Operands are 16-bit matrices in memory with 16-byte aligned rows, read in the direction that they lie in: an operand whose rows run
 // along the summed index is K-major, one whose rows run along the tile's own index is MN-major (the tensor core takes both), so no
